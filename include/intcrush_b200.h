@@ -342,6 +342,76 @@ int ic_piso(const float* W, int64_t M, int64_t N, int64_t ldw, const float* hdia
             int qmin, int qmax, float divisor, const float* coarse, int ncoarse,
             const float* fine, int nfine, float* scales, int8_t* zp, void* stream);
 
+/* ------------------------------- low-precision operands of linear layers */
+/* Formats of quantized rows (no counterpart in the reference, which writes
+ * INT4/INT8 weights and leaves their use to the loader):
+ *   IC_INT8   int8 codes, fp32 scale s per row; value = code * s
+ *   IC_MXFP4  E2M1 codes, one E8M0 byte per 32 columns; value = code * 2^(byte-127)
+ *   IC_NVFP4  E2M1 codes, one E4M3 byte per 16 columns, fp32 scale g per row;
+ *             value = code * e4m3(byte) * g
+ * 4-bit codes: two to a byte, low nibble = even column, rows of kp/2 bytes, kp a
+ * multiple of 32.  Block-scale bytes lie in tiles of 128 rows x 4 blocks, 512
+ * bytes each: row r, block b at byte ((r/128)*ktiles + b/4)*512 + (r%32)*16 +
+ * (r%128/32)*4 + b%4 with ktiles = ceil(blocks/4); the buffer holds
+ * ceil(M/128)*ktiles tiles and the bytes of rows and blocks beyond the matrix
+ * are zero.  Codes and scales are 16-byte aligned.  A value that is not finite
+ * marks its mxfp4 block (byte 255), its nvfp4 row or its int8 row (scale NaN);
+ * the codes there are 0. */
+enum { IC_INT8 = 0, IC_MXFP4 = 1, IC_NVFP4 = 2 };
+
+/* Rows x [M, K] (fp32/fp16/bf16, row pitch ldx) to 4-bit floating point after
+ * the group Hadamard of ic_rotate_weights (rot 0 or a power of two in 16..512;
+ * bit-identical to quantizing its fp32 output).  kp: K rounded up to a multiple
+ * of max(32, rot), the padding zero.  mxfp4: per 32, byte = max(floor(log2 amax)
+ * - 2, -127) + 127.  nvfp4: g = max(amax(row) * (1/2688), 1e-30), or the given
+ * row_scale_in (stride 0: one for all rows, 1: one per row; not positive or not
+ * finite marks the row); per 16, byte = E4M3(amax * (1/(6g))); codes =
+ * E2M1(x * (1/(scale*g))).  Codes round to nearest even and saturate at 6.
+ * row_scale fp32 [M] is written for nvfp4 only. */
+int ic_fp4_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int fmt, int rot,
+                    int64_t kp, const float* row_scale_in, int64_t row_scale_stride, uint8_t* packed,
+                    uint8_t* scales, float* row_scale, void* stream);
+
+/* h = x + residual (residual may be NULL), written to residual_out in x's type
+ * (not overlapping x or residual); y = h / sqrt(mean(h^2) + eps) * weight; the
+ * group Hadamard of y as in ic_fp4_quantize; and the rows in format fmt.
+ * IC_INT8: q = int8 codes [M, kp] of row pitch ldq (a multiple of 16, at least
+ * kp rounded up to 16; the padding is written as 0), kp = K rounded up to a
+ * multiple of rot, row_scale = max(amax * (1/127), 1e-30), codes
+ * round-half-away, sums int32 [M] (or NULL) = the sum of a row's codes.  4-bit
+ * formats: q = packed codes, ldq = kp/2, as ic_fp4_quantize. */
+int ic_rmsnorm_quantize(const void* x, const void* residual, int dtype, int64_t M, int64_t K,
+                        int64_t ldx, int64_t ldr, const void* weight, int weight_dtype, float eps,
+                        int fmt, int rot, int64_t kp, void* residual_out, int64_t ldo, void* q,
+                        int64_t ldq, uint8_t* scales, float* row_scale, int32_t* sums, void* stream);
+
+/* The values of quantized rows, fp32 products rounded once to `dtype`. */
+int ic_fp4_dequantize(const uint8_t* packed, const uint8_t* scales, const float* row_scale, int fmt,
+                      int64_t M, int64_t kp, int dtype, void* out, int64_t ldo, void* stream);
+int ic_int8_dequantize(const int8_t* codes, int64_t ldq, const float* row_scale, int64_t M,
+                       int64_t K, int dtype, void* out, int64_t ldo, void* stream);
+/* sums[i] = sum of row i's codes */
+int ic_int8_row_sums(const int8_t* codes, int64_t ldq, int64_t M, int64_t K, int32_t* sums,
+                     void* stream);
+
+/* y [m, n] = a b^T + bias of two 4-bit operands of one format and kp (block-scaled
+ * tcgen05 products, fp32 accumulation).  bias per column of y (fp32/fp16/bf16) or
+ * NULL; y fp32/fp16/bf16, row pitch ldy. */
+int ic_fp4_matmul(const uint8_t* a_packed, const uint8_t* a_scales, const float* a_row_scale,
+                  const uint8_t* b_packed, const uint8_t* b_scales, const float* b_row_scale, int fmt,
+                  int64_t m, int64_t n, int64_t kp, const void* bias, int bias_dtype, int out_dtype,
+                  void* y, int64_t ldy, void* stream);
+
+/* y [m, n] = (codes w_codes^T - sums w_zp^T) * scales * w_scales + bias: int8 rows
+ * (scale per row) times INT8 weights as ic_rtn_* writes them (fp16 scale and,
+ * asymmetric, int8 zero-point per row; value = (code - zp) * scale), sums exact in
+ * int32.  sums (the row sums of codes) are read when w_zp is given.  Row pitches
+ * multiples of 16, codes 16-byte aligned; k up to 131071, with zero-points 65535. */
+int ic_int8_matmul(const int8_t* codes, int64_t lda, const float* scales, const int32_t* sums,
+                   const int8_t* w_codes, int64_t ldw, const uint16_t* w_scales_f16,
+                   const int8_t* w_zp, int64_t m, int64_t n, int64_t k, const void* bias,
+                   int bias_dtype, int out_dtype, void* y, int64_t ldy, void* stream);
+
 /* ------------------------------------------------------------- utilities */
 /* stats[2] = {sum(row_sqerr)/count, max(row_maxerr)} (fp64) */
 int ic_finalize_stats(const double* row_sqerr, const float* row_maxerr, int64_t M,

@@ -37,3 +37,6 @@ from .permuquant import (  # noqa: E402,F401
     find_permutation_with_acceptance, sweep_alpha,
 )
 from .svd import SVDResult, decompose_weight  # noqa: E402,F401
+from .fp4 import FP4Tensor, dequantize_fp4, matmul_fp4, quantize_fp4  # noqa: E402,F401
+from .int8 import Int8Rows, dequantize_int8, matmul_int8  # noqa: E402,F401
+from .rmsnorm import rmsnorm_quantize  # noqa: E402,F401

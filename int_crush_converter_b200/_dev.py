@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _native as nat
@@ -44,3 +46,8 @@ def split(t32: torch.Tensor, ld: int | None = None):
 
 def workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
+
+
+def on(dev: torch.device):
+    """Context in which ``dev`` is the current device (nothing to enter when it already is)."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)

@@ -29,6 +29,7 @@ IC_ERR_UNSUPPORTED = -6
 IC_ERR_WORKSPACE = -7
 
 IC_F32, IC_F16, IC_BF16 = 0, 1, 2
+IC_INT8, IC_MXFP4, IC_NVFP4 = 0, 1, 2
 
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -85,6 +86,15 @@ SIGNATURES = {
                              _i32, _i32, _vp, _sz, _vp]),
     "ic_piso": (_i32, [_vp, _i64, _i64, _i64, _vp, _i32, _i32, _i32, _f32, _vp, _i32, _vp, _i32, _vp,
                        _vp, _vp]),
+    "ic_fp4_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _i32, _i64, _vp, _i64, _vp, _vp, _vp, _vp]),
+    "ic_rmsnorm_quantize": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _i32, _f32, _i32, _i32, _i64, _vp,
+                                   _i64, _vp, _i64, _vp, _vp, _vp, _vp]),
+    "ic_fp4_dequantize": (_i32, [_vp, _vp, _vp, _i32, _i64, _i64, _i32, _vp, _i64, _vp]),
+    "ic_int8_dequantize": (_i32, [_vp, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp]),
+    "ic_int8_row_sums": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp]),
+    "ic_fp4_matmul": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _i64, _vp]),
+    "ic_int8_matmul": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _i32, _vp,
+                              _i64, _vp]),
     "ic_finalize_stats": (_i32, [_vp, _vp, _i64, _f64, _vp, _vp]),
     "ic_transpose": (_i32, [_vp, _vp, _i64, _i64, _i64, _f32, _vp, _vp, _i64, _vp]),
     "ic_split_tf32": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),

@@ -1,0 +1,506 @@
+// Products of low-precision operands on the 5th-generation tensor cores.
+//
+//   matmul_fp4:   y = (sum_blocks sa*sb * sum_k a*b) * ga * gb + bias   (E2M1 codes; mxfp4 or nvfp4 scales)
+//   matmul_int8:  y = (sum_k a*w - zp * sum_k a) * sa * sw + bias        (exact int32 sums)
+//
+// One CTA computes a 128 x BN tile of the product of its "row" operand P
+// (128 rows) and its "column" operand Q (BN rows), both K-major, 128 bytes of
+// K per stage.  With many rows of activations P = activations; with few
+// (`swap`) P = weights, so that 128 rows of tensor-core work are weight rows
+// and the few activation rows set BN.  Warp roles (256 threads): warp 0 TMA
+// producer, warp 1 MMA issuer, warp 2 TMEM allocator, warps 4-7 epilogue.
+// The 4-bit kinds take their block scales from tensor memory: each stage's
+// scale tiles come by bulk copy, and tcgen05.cp puts them in a ring of TMEM
+// columns as deep as the stage ring, so a slot is rewritten only after the
+// products that read it have finished.
+//
+// With few tiles a cluster of S CTAs splits K; each leaves its partial tile in
+// its own shared memory and the cluster adds them in rank order, so the result
+// does not depend on timing.  All waits are bounded (see common.cuh).
+#include <cstdlib>
+
+#include "internal.h"
+#include "lowp.cuh"
+
+namespace ic {
+namespace {
+
+constexpr int BM = 128;
+constexpr int ROW_BYTES = 128;  // K bytes per stage: one 128-byte swizzle row
+constexpr unsigned long long WAIT_LIMIT_NS = 2000000000ull;
+constexpr int MAX_SPLIT = 8;
+
+struct LowpArgs {
+  int pm, qn;        // rows of P and Q
+  int kbytes;        // bytes of K
+  int ktiles;        // scale tiles (4 blocks) along K
+  int splits;        // CTAs per tile (cluster size)
+  int swap;          // P = weights: the output is transposed on the way out
+  const uint8_t* p_scales;
+  const uint8_t* q_scales;
+  const void* p_row;  // per-row factors: fp32, or fp16 for INT8 weights; null: 1
+  const void* q_row;
+  int p_half, q_half;  // the factors are fp16
+  const int8_t* zp;    // INT8 zero-points of the weights, or null
+  const int32_t* sums; // row sums of the activations
+  const void* bias;    // per weight row
+  int bias_type;
+  void* y;
+  long long ldy;
+  int out_type;
+  unsigned* flags;
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, unsigned* flags) {
+  return mbar_wait_bounded(bar, parity, flags, WAIT_LIMIT_NS);
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+// K-major operand in 128-byte swizzled rows: 8-row groups 1024 bytes apart
+__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)2 << 61;
+}
+// one scale tile, 32 rows of 16 bytes without swizzle: 8-row groups 128 bytes apart
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)8 << 16 | (uint64_t)8 << 32 | (uint64_t)1 << 46;
+}
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+template <int KIND>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                    uint32_t accumulate) {
+  if (KIND == IC_INT8)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else if (KIND == IC_MXFP4)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t saddr, uint32_t rank) {
+  uint32_t out;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(saddr), "r"(rank));
+  return out;
+}
+__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// 16 accumulator columns of this warp's 32 lanes
+#define IC_TMEM_LD16(taddr, r)                                                                                   \
+  asm volatile(                                                                                                  \
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"   \
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),          \
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])     \
+      : "r"(taddr))
+
+template <int KIND, int BN>
+struct Cfg {
+  static constexpr bool FP4 = KIND != IC_INT8;
+  static constexpr int SF_TILES = KIND == IC_NVFP4 ? 4 : KIND == IC_MXFP4 ? 2 : 0;  // scale tiles per stage and 128 rows
+  static constexpr int Q_ATOMS = BN > 128 ? 2 : 1;
+  static constexpr int P_BYTES = BM * ROW_BYTES;
+  static constexpr int Q_BYTES = BN * ROW_BYTES;
+  static constexpr int PS_BYTES = SF_TILES * 512;
+  static constexpr int QS_BYTES = SF_TILES * 512 * Q_ATOMS;
+  static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES + PS_BYTES + QS_BYTES;
+  // narrow tiles leave room for two CTAs on an SM; wide ones take the SM
+  static constexpr int CTAS = BN <= 64 ? 2 : 1;
+  static constexpr int STAGES = (CTAS == 2 ? 98304 : 212992) / STAGE_BYTES;
+  static constexpr int SF_COLS = SF_TILES * 4 * (1 + Q_ATOMS);  // TMEM columns of one stage's scales
+  static constexpr int ACC_COLS = BN < 32 ? 32 : BN;
+  static constexpr int TMEM_NEED = ACC_COLS + STAGES * SF_COLS;
+  static constexpr int TMEM_COLS = TMEM_NEED <= 32 ? 32 : TMEM_NEED <= 64 ? 64 : TMEM_NEED <= 128 ? 128 : TMEM_NEED <= 256 ? 256 : 512;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 /*align*/ + 512 /*barriers*/;
+  static_assert(TMEM_NEED <= 512 / CTAS, "tensor memory");
+  static_assert(BM * BN * 4 <= STAGES * STAGE_BYTES, "a partial tile fits in the stages");
+  static constexpr uint32_t IDESC =
+      KIND == IC_INT8 ? (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24)
+                      : (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | (KIND == IC_MXFP4 ? 1u << 23 : 0u) |
+                            ((uint32_t)(BM >> 4) << 24);
+};
+
+__device__ __forceinline__ float load_any(const void* p, int type, long long i) {
+  if (type == IC_F32) return static_cast<const float*>(p)[i];
+  if (type == IC_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_any(void* p, int type, long long i, float v) {
+  if (type == IC_F32) static_cast<float*>(p)[i] = v;
+  else if (type == IC_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+// y[token, n] of one sum: fp32 scaling in a fixed order, one rounding to the output type at the end
+template <int KIND>
+__device__ __forceinline__ float finish(const LowpArgs& a, uint32_t acc, int token, int n, const void* tok_row, int tok_half,
+                                        const void* w_row, int w_half) {
+  float v;
+  if (KIND == IC_INT8) {
+    int s = (int)acc;
+    if (a.zp) s -= (int)a.zp[n] * a.sums[token];
+    v = (float)s;
+  } else {
+    v = __uint_as_float(acc);
+  }
+  if (tok_row) v = __fmul_rn(v, load_any(tok_row, tok_half ? IC_F16 : IC_F32, token));
+  if (w_row) v = __fmul_rn(v, load_any(w_row, w_half ? IC_F16 : IC_F32, n));
+  if (a.bias) v = __fadd_rn(v, load_any(a.bias, a.bias_type, n));
+  return v;
+}
+
+constexpr int GROUP = 16;  // row tiles per group of the tile order: a wave of CTAs reads a compact patch of P and Q
+
+template <int KIND, int BN>
+__global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
+    lowp_gemm_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ, const LowpArgs a) {
+  using C = Cfg<KIND, BN>;
+  constexpr int STAGES = C::STAGES;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE_BYTES);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 1);
+  auto full_bar = [&](int s) { return smem_u32(bars + s); };
+  auto empty_bar = [&](int s) { return smem_u32(bars + STAGES + s); };
+  const uint32_t acc_bar = smem_u32(bars + 2 * STAGES);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tile = blockIdx.x / a.splits, rank = blockIdx.x - tile * a.splits;
+  const int pt = (a.pm + BM - 1) / BM, qt = (a.qn + BN - 1) / BN;
+  const int per = GROUP * qt, grp = tile / per, first = grp * GROUP, gm = min(GROUP, pt - first), local = tile - grp * per;
+  const int p0 = (first + local % gm) * BM, q0 = (local / gm) * BN;
+  const int stages_all = (a.kbytes + ROW_BYTES - 1) / ROW_BYTES;
+  const int kt0 = (int)((long long)rank * stages_all / a.splits), kt1 = (int)((long long)(rank + 1) * stages_all / a.splits);
+  const int n = kt1 - kt0;  // at least one: the host splits no further than the stages
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(acc_bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(C::TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;");
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0 && lane == 0) {
+    // ---------------- TMA producer ----------------
+    int issued = 0;
+    for (int i = 0; i < n; ++i) {
+      const int s = i % STAGES;
+      if (i >= STAGES && !mbar_wait(empty_bar(s), ((i / STAGES) & 1) ^ 1, a.flags)) break;
+      const int kt = kt0 + i;
+      const uint32_t base = smem_u32(smem + s * C::STAGE_BYTES);
+      uint32_t bytes = C::P_BYTES + C::Q_BYTES, sf = 0;
+      const int rt = q0 >> 7;
+      const bool two = C::Q_ATOMS == 2 && q0 + BM < a.qn;
+      if (C::FP4) {
+        sf = (uint32_t)min(C::SF_TILES, a.ktiles - kt * C::SF_TILES) * 512u;  // at least one tile: kt is within K
+        bytes += sf * (two ? 3u : 2u);
+      }
+      mbar_expect_tx(full_bar(s), bytes);
+      tma_load_2d(base, &tmP, kt * ROW_BYTES, p0, full_bar(s));
+      tma_load_2d(base + C::P_BYTES, &tmQ, kt * ROW_BYTES, q0, full_bar(s));
+      if (C::FP4) {
+        const uint32_t ps = base + C::P_BYTES + C::Q_BYTES, qs = ps + C::PS_BYTES;
+        const long long k = (long long)kt * C::SF_TILES;
+        bulk_load(ps, a.p_scales + ((long long)(p0 >> 7) * a.ktiles + k) * 512, sf, full_bar(s));
+        bulk_load(qs, a.q_scales + ((long long)rt * a.ktiles + k) * 512, sf, full_bar(s));
+        if (two) bulk_load(qs + C::PS_BYTES, a.q_scales + ((long long)(rt + 1) * a.ktiles + k) * 512, sf, full_bar(s));
+      }
+      issued = i + 1;
+    }
+    // no copy of this CTA is in flight when it leaves (already true unless a wait gave up)
+    for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(full_bar(i % STAGES), (i / STAGES) & 1, a.flags);
+  } else if (warp == 1 && lane == 0) {
+    // ---------------- MMA issuer ----------------
+    const uint32_t sf0 = tmem + C::ACC_COLS;
+    const uint32_t qcol = C::FP4 ? (uint32_t)((q0 & 127) >> 5) : 0u;  // narrow tiles start inside a 128-row scale tile
+    for (int i = 0; i < n; ++i) {
+      const int s = i % STAGES;
+      if (!mbar_wait(full_bar(s), (i / STAGES) & 1, a.flags)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;");
+      const uint32_t base = smem_u32(smem + s * C::STAGE_BYTES);
+      const int steps = min(4, (a.kbytes - (kt0 + i) * ROW_BYTES + 31) / 32);  // 32 bytes of K each
+      const uint32_t sfp = sf0 + s * C::SF_COLS, sfq = sfp + C::SF_TILES * 4;
+      if (C::FP4) {
+        const uint32_t ps = base + C::P_BYTES + C::Q_BYTES, qs = ps + C::PS_BYTES;
+        const int tiles = KIND == IC_NVFP4 ? steps : (steps + 1) / 2;
+#pragma unroll
+        for (int t = 0; t < C::SF_TILES; ++t) {
+          if (t >= tiles) break;
+          copy_scales(sfp + t * 4, scale_desc(ps + t * 512));
+#pragma unroll
+          for (int u = 0; u < C::Q_ATOMS; ++u)
+            copy_scales(sfq + (t * C::Q_ATOMS + u) * 4, scale_desc(qs + u * C::PS_BYTES + t * 512));
+        }
+      }
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        if (kk >= steps) break;
+        const int t = KIND == IC_NVFP4 ? kk : kk >> 1;
+        const uint32_t id = KIND == IC_MXFP4 && (kk & 1) ? C::IDESC | (2u << 4) | (2u << 29) : C::IDESC;
+        mma<KIND>(tmem, operand_desc(base + kk * 32), operand_desc(base + C::P_BYTES + kk * 32), id, sfp + t * 4,
+                  sfq + t * C::Q_ATOMS * 4 + qcol, (i | kk) ? 1u : 0u);
+      }
+      mma_commit(empty_bar(s));
+    }
+    mma_commit(acc_bar);
+  }
+  __syncwarp();
+
+  // ---------------- epilogue ----------------
+  const void *tok_row = a.swap ? a.q_row : a.p_row, *w_row = a.swap ? a.p_row : a.q_row;
+  const int tok_half = a.swap ? a.q_half : a.p_half, w_half = a.swap ? a.p_half : a.q_half;
+  const int q = warp & 3;
+  uint32_t* part = reinterpret_cast<uint32_t*>(smem);  // [column][128 rows]
+  if (warp >= 4) {
+    bool ok = mbar_wait(acc_bar, 0, a.flags);
+    if (!ok) mbar_wait(acc_bar, 0, a.flags);  // products in flight end before their tensor memory is freed
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    const int row = p0 + q * 32 + lane;
+    for (int c = 0; c < BN; c += 16) {
+      uint32_t r[16];
+      IC_TMEM_LD16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      if (a.splits > 1) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[(c + j) * BM + q * 32 + lane] = r[j];
+      } else if (ok && row < a.pm) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int col = q0 + c + j;
+          if (col < a.qn) {
+            const int token = a.swap ? col : row, w = a.swap ? row : col;
+            store_any(a.y, a.out_type, (long long)token * a.ldy + w, finish<KIND>(a, r[j], token, w, tok_row, tok_half, w_row, w_half));
+          }
+        }
+      }
+    }
+  }
+  if (a.splits > 1) {
+    cluster_sync();
+    const int c0 = rank * BN / a.splits, c1 = (rank + 1) * BN / a.splits;
+    for (int i = threadIdx.x; i < (c1 - c0) * BM; i += blockDim.x) {
+      const int c = c0 + i / BM, lrow = i % BM, row = p0 + lrow, col = q0 + c;
+      if (row >= a.pm || col >= a.qn) continue;
+      const uint32_t at = smem_u32(part + c * BM + lrow);
+      uint32_t s = 0;
+      float f = 0.f;
+      for (int r = 0; r < a.splits; ++r) {
+        const uint32_t v = ld_cluster(map_to_rank(at, r));
+        if (KIND == IC_INT8) s += v;
+        else f = __fadd_rn(f, __uint_as_float(v));
+      }
+      if (KIND != IC_INT8) s = __float_as_uint(f);
+      const int token = a.swap ? col : row, w = a.swap ? row : col;
+      store_any(a.y, a.out_type, (long long)token * a.ldy + w, finish<KIND>(a, s, token, w, tok_row, tok_half, w_row, w_half));
+    }
+    cluster_sync();  // no CTA leaves while a peer reads its partial tile
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  if (warp == 2) {
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static const EncodeTiledFn fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<EncodeTiledFn>(p);
+    return EncodeTiledFn(nullptr);
+  }();
+  return fn;
+}
+
+int make_map(CUtensorMap* tm, const void* base, int64_t rows, int64_t kbytes, int64_t ld, int box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(IC_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[2] = {(cuuint64_t)kbytes, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {(cuuint32_t)ROW_BYTES, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(IC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) rows=%lld bytes=%lld ld=%lld", (int)r, (long long)rows,
+                (long long)kbytes, (long long)ld);
+  return IC_OK;
+}
+
+struct Operand {
+  const void* codes;
+  int64_t rows, ld;  // ld in bytes
+  const uint8_t* scales;
+  const void* row;
+  int half;
+};
+
+template <int KIND, int BN>
+int launch(const Operand& p, const Operand& q, LowpArgs a, cudaStream_t st) {
+  using C = Cfg<KIND, BN>;
+  static std::atomic<unsigned long long> done{0};
+  IC_TRY(once_per_device(done, [] {
+    IC_CUDA(cudaFuncSetAttribute(lowp_gemm_kernel<KIND, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    return (int)IC_OK;
+  }));
+  CUtensorMap tp, tq;
+  IC_TRY(make_map(&tp, p.codes, p.rows, a.kbytes, p.ld, BM));
+  IC_TRY(make_map(&tq, q.codes, q.rows, a.kbytes, q.ld, BN));
+  a.pm = (int)p.rows, a.qn = (int)q.rows;
+  a.p_scales = p.scales, a.q_scales = q.scales;
+  a.p_row = p.row, a.q_row = q.row, a.p_half = p.half, a.q_half = q.half;
+  const int64_t tiles = cdiv(p.rows, BM) * cdiv(q.rows, BN);
+  const int64_t stages = cdiv(a.kbytes, ROW_BYTES);
+  // split K while the split grid still fits the 148 SMs at once
+  a.splits = 1;
+  while (a.splits < MAX_SPLIT && tiles * a.splits * 2 <= 148 * C::CTAS && stages >= a.splits * 2) a.splits *= 2;
+  if (tiles * a.splits > INT32_MAX) return fail(IC_ERR_UNSUPPORTED, "matmul: too many tiles");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(tiles * a.splits), 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)a.splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  IC_CUDA(cudaLaunchKernelEx(&cfg, lowp_gemm_kernel<KIND, BN>, tp, tq, a));
+  IC_CHECK_LAUNCH();
+  return IC_OK;
+}
+
+// x [m, k] times w [n, k]^T.  Up to 128 activation rows the weights take the
+// 128-row side and the activations a tile as narrow as they are.
+template <int KIND>
+int matmul(const Operand& x, const Operand& w, LowpArgs a, cudaStream_t st) {
+  a.swap = x.rows <= 128;
+  if (!a.swap) return launch<KIND, 128>(x, w, a, st);
+  if (x.rows <= 16) return launch<KIND, 16>(w, x, a, st);
+  if (x.rows <= 32) return launch<KIND, 32>(w, x, a, st);
+  if (x.rows <= 64) return launch<KIND, 64>(w, x, a, st);
+  return launch<KIND, 128>(w, x, a, st);
+}
+
+int check_product(const char* what, int64_t m, int64_t n, int64_t k, const void* bias, int bias_dtype, int out_dtype,
+                  const void* y, int64_t ldy) {
+  if (m < 0 || n < 0 || k <= 0 || ldy < n) return fail(IC_ERR_INVALID, "%s: bad shape", what);
+  if (m > INT32_MAX / 2 || n > INT32_MAX / 2 || k > INT32_MAX / 2) return fail(IC_ERR_UNSUPPORTED, "%s: size", what);
+  if (out_dtype < IC_F32 || out_dtype > IC_BF16 || (bias && (bias_dtype < IC_F32 || bias_dtype > IC_BF16)))
+    return fail(IC_ERR_INVALID, "%s: unknown dtype", what);
+  if (m > 0 && n > 0 && !y) return fail(IC_ERR_INVALID, "%s: null pointer", what);
+  return IC_OK;
+}
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace
+}  // namespace ic
+
+extern "C" int ic_fp4_matmul(const uint8_t* a_packed, const uint8_t* a_scales, const float* a_row_scale,
+                             const uint8_t* b_packed, const uint8_t* b_scales, const float* b_row_scale, int fmt,
+                             int64_t m, int64_t n, int64_t kp, const void* bias, int bias_dtype, int out_dtype, void* y,
+                             int64_t ldy, void* stream) {
+  using namespace ic;
+  if (fmt != IC_MXFP4 && fmt != IC_NVFP4) return fail(IC_ERR_INVALID, "fp4_matmul: unknown format %d", fmt);
+  IC_TRY(check_product("fp4_matmul", m, n, kp, bias, bias_dtype, out_dtype, y, ldy));
+  if (kp % 32) return fail(IC_ERR_INVALID, "fp4_matmul: kp must be a multiple of 32");
+  if (m == 0 || n == 0) return IC_OK;
+  if (!a_packed || !a_scales || !b_packed || !b_scales || (fmt == IC_NVFP4 && (!a_row_scale || !b_row_scale)))
+    return fail(IC_ERR_INVALID, "fp4_matmul: null pointer");
+  if (!aligned16(a_packed) || !aligned16(a_scales) || !aligned16(b_packed) || !aligned16(b_scales))
+    return fail(IC_ERR_INVALID, "fp4_matmul: codes and scales must be 16-byte aligned");
+  LowpArgs a{};
+  a.kbytes = (int)(kp / 2);
+  a.ktiles = (int)fp4_ktiles(fmt, kp);
+  a.bias = bias, a.bias_type = bias_dtype, a.y = y, a.ldy = ldy, a.out_type = out_dtype;
+  a.flags = device_flags();
+  if (!a.flags) return fail(IC_ERR_CUDA, "device status word unavailable");
+  const bool nv = fmt == IC_NVFP4;
+  const Operand x{a_packed, m, kp / 2, a_scales, nv ? a_row_scale : nullptr, 0};
+  const Operand w{b_packed, n, kp / 2, b_scales, nv ? b_row_scale : nullptr, 0};
+  return nv ? matmul<IC_NVFP4>(x, w, a, (cudaStream_t)stream) : matmul<IC_MXFP4>(x, w, a, (cudaStream_t)stream);
+}
+
+extern "C" int ic_int8_matmul(const int8_t* codes, int64_t lda, const float* scales, const int32_t* sums,
+                              const int8_t* w_codes, int64_t ldw, const uint16_t* w_scales_f16, const int8_t* w_zp,
+                              int64_t m, int64_t n, int64_t k, const void* bias, int bias_dtype, int out_dtype, void* y,
+                              int64_t ldy, void* stream) {
+  using namespace ic;
+  IC_TRY(check_product("int8_matmul", m, n, k, bias, bias_dtype, out_dtype, y, ldy));
+  // |sum a*w| <= 2^14 k, and with zero-points |sum a*(w - zp)| and zp * sum a on top of it
+  if (k > (w_zp ? 65535 : 131071)) return fail(IC_ERR_UNSUPPORTED, "int8_matmul: int32 sums hold k up to %d", w_zp ? 65535 : 131071);
+  if (m == 0 || n == 0) return IC_OK;
+  if (!codes || !scales || !w_codes || !w_scales_f16 || (w_zp && !sums)) return fail(IC_ERR_INVALID, "int8_matmul: null pointer");
+  if (lda < k || ldw < k || lda % 16 || ldw % 16 || !aligned16(codes) || !aligned16(w_codes))
+    return fail(IC_ERR_INVALID, "int8_matmul: rows of codes must be 16-byte aligned, with pitches of a multiple of 16");
+  LowpArgs a{};
+  a.kbytes = (int)k;
+  a.zp = w_zp, a.sums = sums;
+  a.bias = bias, a.bias_type = bias_dtype, a.y = y, a.ldy = ldy, a.out_type = out_dtype;
+  a.flags = device_flags();
+  if (!a.flags) return fail(IC_ERR_CUDA, "device status word unavailable");
+  const Operand x{codes, m, lda, nullptr, scales, 0};
+  const Operand w{w_codes, n, ldw, nullptr, w_scales_f16, 1};
+  return matmul<IC_INT8>(x, w, a, (cudaStream_t)stream);
+}

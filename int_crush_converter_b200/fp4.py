@@ -1,0 +1,234 @@
+"""Microscaled 4-bit floating point on the GPU: quantization, values, product.
+
+Two formats of E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives):
+
+* ``"mxfp4"``: one power-of-two scale per 32 columns;
+* ``"nvfp4"``: one E4M3 scale per 16 columns and one fp32 scale per row.
+
+Weights and activations are quantized the same way, after the same group
+Hadamard rotation that the INT4 path uses (``rot_size``), and multiplied on the
+block-scaled tensor cores.  Nothing here has a gradient.
+"""
+
+from __future__ import annotations
+
+import dataclasses
+
+import torch
+
+from . import _native as nat
+from ._dev import back, device_of, on
+from .rotation import _DT, _is_power_of_two, _rotate_rows
+
+FORMATS = {"mxfp4": nat.IC_MXFP4, "nvfp4": nat.IC_NVFP4}
+BLOCK = {"mxfp4": 32, "nvfp4": 16}
+
+
+def _ktiles(fmt: str, kp: int) -> int:
+    return -(-kp // (4 * BLOCK[fmt]))
+
+
+@dataclasses.dataclass
+class FP4Tensor:
+    """Rows in a 4-bit floating-point format.
+
+    ``packed``: uint8 [rows, columns/2], low nibble = even column; columns are the
+    input's, padded with zeros to a multiple of 32 (and of the rotation size).
+    ``scales``: the block-scale bytes, uint8 [ceil(rows/128), ceil(blocks/4), 32, 4, 4]:
+    row r, block b at [r//128, b//4, r%32, r%128//32, b%4] (the order in which the
+    product reads them; :meth:`block_scales` gives them row by row).
+    ``row_scale``: fp32 [rows] (nvfp4), else None.
+    ``lead``: the leading dimensions of the tensor that was quantized (default [rows]).
+    """
+
+    packed: torch.Tensor
+    scales: torch.Tensor
+    row_scale: torch.Tensor | None
+    fmt: str = "mxfp4"
+    in_features: int | None = None
+    rot_size: int = 0
+    lead: tuple | None = None
+
+    @property
+    def rows(self) -> int:
+        return self.packed.shape[0]
+
+    @property
+    def columns(self) -> int:
+        return self.packed.shape[1] * 2
+
+    @property
+    def device(self) -> torch.device:
+        return self.packed.device
+
+    def to(self, device) -> "FP4Tensor":
+        move = lambda t: None if t is None else t.to(device)  # noqa: E731
+        return dataclasses.replace(self, packed=move(self.packed), scales=move(self.scales), row_scale=move(self.row_scale))
+
+    def block_scales(self) -> torch.Tensor:
+        """The block-scale bytes as uint8 [rows, blocks]."""
+        a, b = self.scales.shape[:2]
+        t = self.scales.permute(0, 3, 2, 1, 4).reshape(a * 128, b * 4)
+        return t[:self.rows, :self.columns // BLOCK[self.fmt]].contiguous()
+
+    def check(self, what: str) -> None:
+        """ValueError unless the parts have the types and sizes the kernels read."""
+        if self.fmt not in FORMATS:
+            raise ValueError(f"{what}: fmt must be one of {sorted(FORMATS)}, got {self.fmt!r}")
+        p, s, g = self.packed, self.scales, self.row_scale
+        if p.dim() != 2 or p.dtype != torch.uint8 or s.dtype != torch.uint8:
+            raise ValueError(f"{what}: packed must be uint8 [rows, columns/2] and scales uint8")
+        rows, kp = p.shape[0], p.shape[1] * 2
+        if kp % 32:
+            raise ValueError(f"{what}: the number of columns must be a multiple of 32, got {kp}")
+        tiles = -(-rows // 128) * _ktiles(self.fmt, kp)
+        if s.numel() != tiles * 512:
+            raise ValueError(f"{what}: {rows} rows of {kp} {self.fmt} columns have {tiles * 512} scale bytes, got {s.numel()}")
+        if (g is None) != (self.fmt == "mxfp4"):
+            raise ValueError(f"{what}: nvfp4 has row scales and mxfp4 none")
+        if g is not None and (g.dtype != torch.float32 or g.numel() != rows or g.device != p.device):
+            raise ValueError(f"{what}: row_scale must be fp32 [rows] on the codes' device")
+        if s.device != p.device:
+            raise ValueError(f"{what}: packed and scales must be on one device")
+        if not p.is_contiguous() or not s.is_contiguous() or (g is not None and not g.is_contiguous()):
+            raise ValueError(f"{what}: packed, scales and row_scale must be contiguous")
+        if (p.data_ptr() | s.data_ptr()) & 15:
+            raise ValueError(f"{what}: packed and scales must be 16-byte aligned")
+
+    def lead_shape(self) -> tuple:
+        return (self.rows,) if self.lead is None else tuple(self.lead)
+
+
+def empty_fp4(rows: int, columns: int, fmt: str, dev: torch.device, **kw) -> FP4Tensor:
+    """An FP4Tensor of uninitialised parts."""
+    return FP4Tensor(torch.empty(rows, columns // 2, dtype=torch.uint8, device=dev),
+                     torch.empty(-(-rows // 128), _ktiles(fmt, columns), 32, 4, 4, dtype=torch.uint8, device=dev),
+                     torch.empty(rows, dtype=torch.float32, device=dev) if fmt == "nvfp4" else None, fmt, **kw)
+
+
+def padded_columns(k: int, fmt: str, rot_size: int) -> int:
+    """Columns held: ``k`` up to whole rotation groups and, for the 4-bit formats, whole runs of 32."""
+    unit = max(rot_size, 1 if fmt == "int8" else 32)
+    return -(-k // unit) * unit
+
+
+def as_rows(x: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """[..., K] -> 2-D rows on ``dev`` with unit column stride (a view where possible)."""
+    x2 = x.to(dev).reshape(-1, x.shape[-1]) if x.dim() != 2 else x.to(dev)
+    if x2.shape[0] and x2.shape[1] and (x2.stride(1) != 1 or x2.stride(0) < x2.shape[1]):
+        x2 = x2.contiguous()
+    return x2
+
+
+def pitch(x2: torch.Tensor) -> int:
+    return max(x2.stride(0), x2.shape[1])
+
+
+def quantize_fp4(x: torch.Tensor, fmt: str = "mxfp4", rot_size: int = 0,
+                 row_scale: torch.Tensor | float | None = None) -> FP4Tensor:
+    """Quantize [..., K] weights or activations (fp32/fp16/bf16) to ``fmt``.
+
+    ``rot_size``: 0, or a power of two: the group Hadamard of ``rotate_weights``
+    first, in fp32 (fused for 16..512).  ``row_scale`` (nvfp4): the second-level
+    scale, one number for all rows or fp32 [rows]; by default each row's
+    max|x|/2688, so that a row does not depend on its neighbours.  A value that is
+    not finite marks its mxfp4 block or its nvfp4 row as NaN.
+    """
+    if fmt not in FORMATS:
+        raise ValueError(f"fmt must be one of {sorted(FORMATS)}, got {fmt!r}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("quantize_fp4 needs at least one column")
+    if rot_size and not _is_power_of_two(rot_size):
+        raise ValueError(f"rot_size must be 0 or a power of 2, got {rot_size}")
+    if x.dtype not in _DT:
+        raise ValueError(f"x must be float32, float16 or bfloat16, got {x.dtype}")
+    if row_scale is not None and fmt != "nvfp4":
+        raise ValueError("row_scale is for nvfp4")
+    dev = device_of(x)
+    lead, k = tuple(x.shape[:-1]), x.shape[-1]
+    x2 = as_rows(x, dev)
+    rows, rot = x2.shape[0], rot_size
+    stride = 0
+    if row_scale is not None:
+        row_scale = torch.as_tensor(row_scale, dtype=torch.float32, device=dev).reshape(-1).contiguous()
+        if row_scale.numel() not in (1, rows):
+            raise ValueError(f"row_scale must have 1 or {rows} values, got {row_scale.numel()}")
+        stride = int(row_scale.numel() == rows and rows > 1)
+    with on(dev):
+        if rot and not 16 <= rot <= 512:
+            x2 = _rotate_rows(x2, rot, dev) if rows else x2.new_empty(0, padded_columns(k, "int8", rot))
+            rot = 0
+        out = empty_fp4(rows, padded_columns(x2.shape[1], fmt, rot), fmt, dev, in_features=k, rot_size=rot_size, lead=lead)
+        if rows:
+            nat.check(nat.load().ic_fp4_quantize(
+                x2.data_ptr(), _DT[x2.dtype], rows, x2.shape[1], pitch(x2), FORMATS[fmt], rot, out.columns,
+                nat.ptr(row_scale), stride, out.packed.data_ptr(), out.scales.data_ptr(), nat.ptr(out.row_scale),
+                nat.stream_ptr(dev)), "quantize_fp4")
+    return out if x.is_cuda else out.to(x.device)
+
+
+def dequantize_fp4(q: FP4Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of ``q``, [lead..., columns] (padding included), in fp32/fp16/bf16."""
+    q.check("dequantize_fp4")
+    if dtype not in _DT:
+        raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+    dev = device_of(q.packed)
+    d = q.to(dev)
+    out = torch.empty(d.rows, d.columns, dtype=dtype, device=dev)
+    if out.numel():
+        with on(dev):
+            nat.check(nat.load().ic_fp4_dequantize(
+                d.packed.data_ptr(), d.scales.data_ptr(), nat.ptr(d.row_scale), FORMATS[q.fmt], d.rows, d.columns,
+                _DT[dtype], out.data_ptr(), d.columns, nat.stream_ptr(dev)), "dequantize_fp4")
+    return back(out.reshape(*q.lead_shape(), d.columns), q.packed)
+
+
+def check_bias(bias: torch.Tensor | None, n: int, dev: torch.device) -> torch.Tensor | None:
+    if bias is None:
+        return None
+    if bias.numel() != n or bias.dtype not in _DT:
+        raise ValueError(f"bias must have {n} values in float32, float16 or bfloat16")
+    return bias.to(dev).reshape(-1).contiguous()
+
+
+def matmul_fp4(a: FP4Tensor, b: FP4Tensor, bias: torch.Tensor | None = None,
+               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``a @ b.T + bias``: activations [lead..., K] times weights [N, K], both in one format.
+
+    Products of codes and scales are exact, their sums and the bias are held in
+    fp32 and rounded once to ``out_dtype`` (fp32/fp16/bf16).  ``b``'s rows are the
+    output's columns.
+    """
+    a.check("matmul_fp4")
+    b.check("matmul_fp4")
+    if a.fmt != b.fmt or a.columns != b.columns:
+        raise ValueError(f"matmul_fp4: operands differ: {a.fmt} with {a.columns} columns, {b.fmt} with {b.columns}")
+    if a.rot_size != b.rot_size:
+        raise ValueError(f"matmul_fp4: operands are rotated by {a.rot_size} and {b.rot_size}")
+    if a.in_features is not None and b.in_features is not None and a.in_features != b.in_features:
+        raise ValueError(f"matmul_fp4: operands have {a.in_features} and {b.in_features} input features")
+    if a.device != b.device:
+        raise ValueError("matmul_fp4: operands are on different devices")
+    if out_dtype not in _DT:
+        raise ValueError(f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
+    dev = device_of(a.packed)
+    m, n = a.rows, b.rows
+    bias_d = check_bias(bias, n, dev)
+    on_cpu = not a.packed.is_cuda
+    if on_cpu:
+        da, db = a.to(dev), b.to(dev)
+    else:
+        da, db = a, b
+    y = torch.empty(m, n, dtype=out_dtype, device=dev)
+    if m and n:
+        if a.columns == 0:
+            y.zero_() if bias_d is None else y.copy_(bias_d.float().expand(m, n))
+        else:
+            with on(dev):
+                nat.check(nat.load().ic_fp4_matmul(
+                    da.packed.data_ptr(), da.scales.data_ptr(), nat.ptr(da.row_scale), db.packed.data_ptr(),
+                    db.scales.data_ptr(), nat.ptr(db.row_scale), FORMATS[a.fmt], m, n, a.columns, nat.ptr(bias_d),
+                    0 if bias_d is None else _DT[bias_d.dtype], _DT[out_dtype], y.data_ptr(), n, nat.stream_ptr(dev)),
+                    "matmul_fp4")
+    y = y.reshape(*a.lead_shape(), n)
+    return y.to(a.device) if on_cpu else y

@@ -1,0 +1,156 @@
+"""INT8 rows (one fp32 scale per row) and their product with INT8 weights on the GPU.
+
+The weights are the codes, fp16 scales and zero-points that ``scales`` and
+``gptq`` write (value = (code - zero_point) * scale); the rows come from
+``rmsnorm_quantize``.  Nothing here has a gradient.
+"""
+
+from __future__ import annotations
+
+import dataclasses
+
+import torch
+
+from . import _native as nat
+from ._dev import back, device_of, on
+from .fp4 import check_bias
+from .rotation import _DT
+
+MAX_K = 131071      # int32 sums of products
+MAX_K_ASYM = 65535  # with zero-points
+
+
+@dataclasses.dataclass
+class Int8Rows:
+    """``codes``: int8 [rows, columns] (columns contiguous; a row pitch of a multiple
+    of 16 bytes is read in place); ``scales``: fp32 [rows, 1]; ``sums``: int32 [rows],
+    the sum of each row's codes (asked for by asymmetric weights), or None."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    sums: torch.Tensor | None = None
+    in_features: int | None = None
+    rot_size: int = 0
+    lead: tuple | None = None
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def columns(self) -> int:
+        return self.codes.shape[1]
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def lead_shape(self) -> tuple:
+        return (self.rows,) if self.lead is None else tuple(self.lead)
+
+    def check(self, what: str) -> None:
+        if self.codes.dim() != 2 or self.codes.dtype != torch.int8:
+            raise ValueError(f"{what}: codes must be int8 [rows, columns]")
+        if self.scales.dtype != torch.float32 or self.scales.numel() != self.rows:
+            raise ValueError(f"{what}: scales must be fp32 [rows, 1]")
+        if self.sums is not None and (self.sums.dtype != torch.int32 or self.sums.numel() != self.rows):
+            raise ValueError(f"{what}: sums must be int32 [rows]")
+        if self.scales.device != self.device or (self.sums is not None and self.sums.device != self.device):
+            raise ValueError(f"{what}: codes, scales and sums must be on one device")
+
+
+def empty_int8(rows: int, columns: int, dev: torch.device, **kw) -> Int8Rows:
+    """Int8Rows of uninitialised parts, rows at a pitch of a multiple of 16 bytes."""
+    buf = torch.empty(rows, (columns + 15) & ~15, dtype=torch.int8, device=dev)
+    return Int8Rows(buf[:, :columns], torch.empty(rows, 1, dtype=torch.float32, device=dev),
+                    torch.empty(rows, dtype=torch.int32, device=dev), **kw)
+
+
+def pitched(codes: torch.Tensor, dev: torch.device) -> tuple[torch.Tensor, int]:
+    """(codes on ``dev`` as the product reads them, row pitch): 16-byte aligned rows,
+    copied when they are not."""
+    c = codes.to(dev)
+    rows, k = c.shape
+    if (k == 1 or c.stride(1) == 1) and c.data_ptr() % 16 == 0:
+        if rows == 1:
+            return c, (k + 15) & ~15
+        if c.stride(0) % 16 == 0 and c.stride(0) >= k:
+            return c, c.stride(0)
+    buf = torch.zeros(rows, (k + 15) & ~15, dtype=torch.int8, device=dev)
+    buf[:, :k] = c
+    return buf, buf.shape[1]
+
+
+def dequantize_int8(q: Int8Rows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of ``q``, [lead..., columns], in fp32/fp16/bf16."""
+    q.check("dequantize_int8")
+    if dtype not in _DT:
+        raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+    dev = device_of(q.codes)
+    out = torch.empty(q.rows, q.columns, dtype=dtype, device=dev)
+    if out.numel():
+        with on(dev):
+            codes = q.codes.to(dev)
+            if codes.stride(1) != 1 or codes.stride(0) < q.columns:
+                codes = codes.contiguous()
+            scales = q.scales.to(dev).reshape(-1).contiguous()
+            nat.check(nat.load().ic_int8_dequantize(
+                codes.data_ptr(), max(codes.stride(0), q.columns), scales.data_ptr(), q.rows, q.columns, _DT[dtype],
+                out.data_ptr(), q.columns, nat.stream_ptr(dev)), "dequantize_int8")
+    return back(out.reshape(*q.lead_shape(), q.columns), q.codes)
+
+
+def matmul_int8(a: Int8Rows, w_codes: torch.Tensor, w_scales: torch.Tensor,
+                w_zero_points: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``a @ W.T + bias`` with W = (w_codes - w_zero_points) * w_scales.
+
+    ``w_codes``: int8 [N, columns] as the quantizers return them (INT4 codes in
+    int8 serve too); ``w_scales``: fp16 [N] or [N, 1]; ``w_zero_points``: int8 or
+    None.  Sums are exact in int32 (columns up to 131071, with zero-points 65535),
+    the scaling and the bias fp32, rounded once to ``out_dtype``.  Weights whose
+    rows are not 16-byte aligned are copied on every call: keep them at such a
+    pitch.
+    """
+    a.check("matmul_int8")
+    if w_codes.dim() != 2 or w_codes.dtype != torch.int8:
+        raise ValueError("matmul_int8: w_codes must be int8 [out, columns]")
+    m, (n, k) = a.rows, w_codes.shape
+    if a.columns != k:
+        raise ValueError(f"matmul_int8: rows have {a.columns} columns, the weights {k}")
+    if k > (MAX_K if w_zero_points is None else MAX_K_ASYM):
+        raise ValueError(f"matmul_int8: int32 sums hold {MAX_K} columns, {MAX_K_ASYM} with zero-points; got {k}")
+    if w_scales.dtype != torch.float16 or w_scales.numel() != n:
+        raise ValueError(f"matmul_int8: w_scales must be float16 with {n} values (one per row)")
+    if w_zero_points is not None and (w_zero_points.dtype != torch.int8 or w_zero_points.numel() != n):
+        raise ValueError(f"matmul_int8: w_zero_points must be int8 with {n} values (one per row)")
+    if out_dtype not in _DT:
+        raise ValueError(f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
+    if any(t is not None and t.device != a.device for t in (w_codes, w_scales, w_zero_points)):
+        raise ValueError("matmul_int8: operands are on different devices")
+    dev = device_of(a.codes)
+    bias_d = check_bias(bias, n, dev)
+    y = torch.empty(m, n, dtype=out_dtype, device=dev)
+    if m and n:
+        if k == 0:
+            y.zero_() if bias_d is None else y.copy_(bias_d.float().expand(m, n))
+        else:
+            with on(dev):
+                st, lib = nat.stream_ptr(dev), nat.load()
+                x, ldx = pitched(a.codes, dev)
+                w, ldw = pitched(w_codes, dev)
+                s = a.scales.to(dev).reshape(-1).contiguous()
+                ws = w_scales.to(dev).reshape(-1).contiguous()
+                zp = sums = None
+                if w_zero_points is not None:
+                    zp = w_zero_points.to(dev).reshape(-1).contiguous()
+                    if a.sums is None:
+                        sums = torch.empty(m, dtype=torch.int32, device=dev)
+                        nat.check(lib.ic_int8_row_sums(x.data_ptr(), ldx, m, k, sums.data_ptr(), st), "matmul_int8")
+                    else:
+                        sums = a.sums.to(dev).reshape(-1).contiguous()
+                nat.check(lib.ic_int8_matmul(
+                    x.data_ptr(), ldx, s.data_ptr(), nat.ptr(sums), w.data_ptr(), ldw, ws.data_ptr(), nat.ptr(zp), m, n, k,
+                    nat.ptr(bias_d), 0 if bias_d is None else _DT[bias_d.dtype], _DT[out_dtype], y.data_ptr(), n, st),
+                    "matmul_int8")
+    return back(y.reshape(*a.lead_shape(), n), a.codes)
