@@ -352,6 +352,331 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
 }
 
 // ---------------------------------------------------------------------------
+// CTA pairs (cta_group::2) for large products: a cluster of two CTAs computes
+// 256 x 256 tiles, one after another, each CTA staging its own 128 rows of P
+// and of Q and the scales of its P rows and of all Q rows.  Per SM and 128
+// bytes of K that is 32 KB of operands for 512 tensor-core cycles; a single
+// CTA's 128 x 128 tile needs 32 KB for 256, more than L2 delivers.
+// The accumulator takes 256 of the 512 TMEM columns and the scales most of the
+// rest, so it is not doubled: eight epilogue warps move it to registers at
+// once (128 columns each), release it, and scale, convert and store while the
+// next tile's products run.
+//   full[s]  leader only: the bytes of both CTAs' loads
+//   empty[s] in each CTA: the commit of the products that read the stage
+//   accf     in each CTA: the commit of a tile's last product
+//   acce     leader only: 16 epilogue warps have taken the accumulator
+constexpr int PAIR_GROUP = 8;  // 256-row tiles per group of the tile order
+
+template <int KIND>
+struct PairCfg {
+  static constexpr bool FP4 = KIND != IC_INT8;
+  static constexpr int BN = 256;
+  static constexpr int SF_TILES = KIND == IC_NVFP4 ? 4 : KIND == IC_MXFP4 ? 2 : 0;
+  static constexpr int P_BYTES = 128 * ROW_BYTES, Q_BYTES = 128 * ROW_BYTES;
+  static constexpr int PS_BYTES = SF_TILES * 512, QS_BYTES = 2 * PS_BYTES;
+  static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES + PS_BYTES + QS_BYTES;
+  static constexpr int STAGES = 4;
+  static constexpr int SF_COLS = SF_TILES * 12;
+  static constexpr int TMEM_COLS = 512;
+  static constexpr int OUT_BYTES = 8 * 4096;      // per epilogue warp: 32 rows of 128 bytes
+  static constexpr int FACTOR_BYTES = 8 * 1024;   // per epilogue warp: 128 column factors and biases
+  static constexpr int SMEM = STAGES * STAGE_BYTES + OUT_BYTES + FACTOR_BYTES + 1024 + 256;
+  static_assert(BN + STAGES * SF_COLS <= TMEM_COLS, "tensor memory");
+  static_assert(SMEM <= 232448, "shared memory");
+  static constexpr uint32_t IDESC =
+      KIND == IC_INT8 ? (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(256 >> 4) << 24)
+                      : (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | (KIND == IC_MXFP4 ? 1u << 23 : 0u) |
+                            ((uint32_t)(256 >> 4) << 24);
+};
+
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* tm, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* tm, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+template <int KIND>
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                         uint32_t accumulate) {
+  if (KIND == IC_INT8)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else if (KIND == IC_MXFP4)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
+  const uint16_t mask = 3;
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(mask)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void remote_arrive(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+#define IC_TMEM_LD32(taddr, r)                                                                   \
+  asm volatile(                                                                                  \
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"   \
+      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"         \
+      : "=r"((r)[0]), "=r"((r)[1]), "=r"((r)[2]), "=r"((r)[3]), "=r"((r)[4]), "=r"((r)[5]),      \
+        "=r"((r)[6]), "=r"((r)[7]), "=r"((r)[8]), "=r"((r)[9]), "=r"((r)[10]), "=r"((r)[11]),    \
+        "=r"((r)[12]), "=r"((r)[13]), "=r"((r)[14]), "=r"((r)[15]), "=r"((r)[16]), "=r"((r)[17]), \
+        "=r"((r)[18]), "=r"((r)[19]), "=r"((r)[20]), "=r"((r)[21]), "=r"((r)[22]), "=r"((r)[23]), \
+        "=r"((r)[24]), "=r"((r)[25]), "=r"((r)[26]), "=r"((r)[27]), "=r"((r)[28]), "=r"((r)[29]), \
+        "=r"((r)[30]), "=r"((r)[31])                                                             \
+      : "r"(taddr))
+
+// One warp's 32 rows x 128 columns of finished sums to y.  `out` is the warp's
+// 4 KB of shared memory: rows of 128 bytes, 16-byte pieces XOR-swizzled by the
+// row, written one row per lane and read back eight lanes to a row, so that
+// global stores cover whole 128-byte lines.
+template <int KIND, typename T>
+__device__ __forceinline__ void store_block(const LowpArgs& a, const uint32_t (&acc)[128], unsigned char* out,
+                                            const float* factor, const float* bias, float rowf, int row0,
+                                            int col0, int lane) {
+  constexpr int G = 128 / sizeof(T);  // columns per pass
+  constexpr int V = 16 / sizeof(T);
+  T* y = static_cast<T*>(a.y);
+  const bool vec = (reinterpret_cast<uintptr_t>(y) & 15) == 0 && (a.ldy * (long long)sizeof(T)) % 16 == 0;
+#pragma unroll
+  for (int g = 0; g < 128 / G; ++g) {
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      uint4 piece;
+      T* e = reinterpret_cast<T*>(&piece);
+#pragma unroll
+      for (int u = 0; u < V; ++u) {
+        const int c = g * G + p * V + u;
+        float v;
+        if (KIND == IC_INT8) v = (float)(int)acc[c];
+        else v = __uint_as_float(acc[c]);
+        if (KIND != IC_MXFP4) v = __fmul_rn(__fmul_rn(v, rowf), factor[c]);
+        if (a.bias) v = __fadd_rn(v, bias[c]);
+        if constexpr (sizeof(T) == 4) e[u] = v;
+        else if constexpr (std::is_same<T, __half>::value) e[u] = __float2half_rn(v);
+        else e[u] = __float2bfloat16_rn(v);
+      }
+      *reinterpret_cast<uint4*>(out + lane * 128 + ((p ^ (lane & 7)) << 4)) = piece;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3), p = lane & 7;
+      const uint4 piece = *reinterpret_cast<const uint4*>(out + r * 128 + ((p ^ (r & 7)) << 4));
+      const int col = col0 + g * G + p * V;
+      if (row0 + r < a.pm && col < a.qn) {
+        T* to = y + (long long)(row0 + r) * a.ldy + col;
+        if (vec && col + V <= a.qn) {
+          *reinterpret_cast<uint4*>(to) = piece;
+        } else {
+          const T* e = reinterpret_cast<const T*>(&piece);
+          for (int u = 0; u < V && col + u < a.qn; ++u) to[u] = e[u];
+        }
+      }
+    }
+    __syncwarp();
+  }
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(384, 1)
+    lowp_pair_kernel(const __grid_constant__ CUtensorMap tmP, const __grid_constant__ CUtensorMap tmQ,
+                     const __grid_constant__ CUtensorMap tmPS, const __grid_constant__ CUtensorMap tmQS, const LowpArgs a) {
+  using C = PairCfg<KIND>;
+  constexpr int STAGES = C::STAGES;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* out_smem = smem + STAGES * C::STAGE_BYTES;
+  float* factor_smem = reinterpret_cast<float*>(out_smem + C::OUT_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(out_smem + C::OUT_BYTES + C::FACTOR_BYTES);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 2);
+  auto full_bar = [&](int s) { return smem_u32(bars + s); };
+  auto empty_bar = [&](int s) { return smem_u32(bars + STAGES + s); };
+  const uint32_t accf = smem_u32(bars + 2 * STAGES), acce = smem_u32(bars + 2 * STAGES + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const int pt = (a.pm + 255) / 256, qt = (a.qn + C::BN - 1) / C::BN, tiles = pt * qt;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int n = (a.kbytes + ROW_BYTES - 1) / ROW_BYTES;
+  auto place = [&](int tile, int& p0, int& q0) {
+    const int per = PAIR_GROUP * qt, grp = tile / per, first = grp * PAIR_GROUP, gm = min(PAIR_GROUP, pt - first);
+    const int local = tile - grp * per;
+    p0 = (first + local % gm) * 256;
+    q0 = (local / gm) * C::BN;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(accf, 1);
+    mbar_init(acce, 16);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(C::TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;");
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0 && lane == 0) {
+    // ---------------- TMA producer (both CTAs) ----------------
+    int g = 0;
+    bool ok = true;
+    for (int tile = pair; tile < tiles && ok; tile += pairs) {
+      int p0, q0;
+      place(tile, p0, q0);
+      for (int i = 0; i < n; ++i, ++g) {
+        const int s = g % STAGES;
+        if (g >= STAGES && !mbar_wait(empty_bar(s), ((g / STAGES) & 1) ^ 1, a.flags)) {
+          ok = false;
+          break;
+        }
+        if (leader) mbar_expect_tx(full_bar(s), 2 * C::STAGE_BYTES);
+        const uint32_t fb = map_to_rank(full_bar(s), 0);
+        const uint32_t base = smem_u32(smem + s * C::STAGE_BYTES);
+        tma_load_2d_pair(base, &tmP, i * ROW_BYTES, p0 + (int)rank * 128, fb);
+        tma_load_2d_pair(base + C::P_BYTES, &tmQ, i * ROW_BYTES, q0 + (int)rank * 128, fb);
+        if (C::FP4) {
+          const uint32_t ps = base + C::P_BYTES + C::Q_BYTES;
+          tma_load_3d_pair(ps, &tmPS, 0, i * C::SF_TILES, (p0 >> 7) + (int)rank, fb);
+          tma_load_3d_pair(ps + C::PS_BYTES, &tmQS, 0, i * C::SF_TILES, q0 >> 7, fb);
+        }
+      }
+    }
+    // no copy is in flight when the pair leaves (already true unless a wait gave up)
+    if (leader)
+      for (int i = max(0, g - STAGES); i < g; ++i) mbar_wait(full_bar(i % STAGES), (i / STAGES) & 1, a.flags);
+  } else if (warp == 1 && lane == 0 && leader) {
+    // ---------------- MMA issuer (leader) ----------------
+    int g = 0, t = 0;
+    bool ok = true;
+    for (int tile = pair; tile < tiles && ok; tile += pairs, ++t) {
+      if (t > 0 && !mbar_wait(acce, (t & 1) ^ 1, a.flags)) break;
+      asm volatile("tcgen05.fence::after_thread_sync;");
+      for (int i = 0; i < n; ++i, ++g) {
+        const int s = g % STAGES;
+        if (!mbar_wait(full_bar(s), (g / STAGES) & 1, a.flags)) {
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        const uint32_t base = smem_u32(smem + s * C::STAGE_BYTES);
+        const int steps = min(4, (a.kbytes - i * ROW_BYTES + 31) / 32);
+        const uint32_t sfp = tmem + C::BN + s * C::SF_COLS, sfq = sfp + C::SF_TILES * 4;
+        if (C::FP4) {
+          const uint32_t ps = base + C::P_BYTES + C::Q_BYTES, qs = ps + C::PS_BYTES;
+#pragma unroll
+          for (int k = 0; k < C::SF_TILES; ++k) {
+            copy_scales_pair(sfp + k * 4, scale_desc(ps + k * 512));
+            copy_scales_pair(sfq + k * 8, scale_desc(qs + k * 512));
+            copy_scales_pair(sfq + k * 8 + 4, scale_desc(qs + C::PS_BYTES + k * 512));
+          }
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          if (kk >= steps) break;
+          const int k = KIND == IC_NVFP4 ? kk : kk >> 1;
+          const uint32_t id = KIND == IC_MXFP4 && (kk & 1) ? C::IDESC | (2u << 4) | (2u << 29) : C::IDESC;
+          mma_pair<KIND>(tmem, operand_desc(base + kk * 32), operand_desc(base + C::P_BYTES + kk * 32), id, sfp + k * 4,
+                         sfq + k * 8, (i | kk) ? 1u : 0u);
+        }
+        mma_commit_pair(empty_bar(s));
+      }
+      mma_commit_pair(accf);
+    }
+  } else if (warp >= 4) {
+    // ---------------- epilogue (both CTAs, own rows) ----------------
+    const int q = warp & 3, h = (warp - 4) >> 2, ew = warp - 4;
+    unsigned char* out = out_smem + ew * 4096;
+    float* factor = factor_smem + ew * 256;  // [128] factors, [128] biases
+    int t = 0;
+    for (int tile = pair; tile < tiles; tile += pairs, ++t) {
+      int p0, q0;
+      place(tile, p0, q0);
+      const int row0 = p0 + (int)rank * 128 + q * 32, row = row0 + lane, col0 = q0 + h * 128;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = i * 32 + lane, col = col0 + c;
+        factor[c] = a.q_row && col < a.qn ? load_any(a.q_row, a.q_half ? IC_F16 : IC_F32, col) : 0.f;
+        factor[128 + c] = a.bias && col < a.qn ? load_any(a.bias, a.bias_type, col) : 0.f;
+      }
+      const float rowf = a.p_row && row < a.pm ? load_any(a.p_row, a.p_half ? IC_F16 : IC_F32, row) : 0.f;
+      __syncwarp();
+      bool ok = mbar_wait(accf, t & 1, a.flags);
+      if (!ok) mbar_wait(accf, t & 1, a.flags);  // products in flight end before their tensor memory is freed
+      asm volatile("tcgen05.fence::after_thread_sync;");
+      uint32_t acc[128];
+      const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * 128);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) IC_TMEM_LD32(at + i * 32, acc + i * 32);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;");
+      __syncwarp();
+      if (lane == 0) remote_arrive(map_to_rank(acce, 0));
+      if (!ok) break;
+      if (KIND == IC_INT8 && a.zp) {
+        const int sum = row < a.pm ? a.sums[row] : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int col = col0 + i * 32 + lane, z = col < a.qn ? a.zp[col] : 0;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[i * 32 + j] -= (uint32_t)(__shfl_sync(0xffffffffu, z, j) * sum);
+        }
+      }
+      if (a.out_type == IC_BF16) store_block<KIND, __nv_bfloat16>(a, acc, out, factor, factor + 128, rowf, row0, col0, lane);
+      else if (a.out_type == IC_F16) store_block<KIND, __half>(a, acc, out, factor, factor + 128, rowf, row0, col0, lane);
+      else store_block<KIND, float>(a, acc, out, factor, factor + 128, rowf, row0, col0, lane);
+    }
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while its peer may still signal its barriers or read its operands
+  if (warp == 2) {
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS));
+  }
+}
+
+// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -431,11 +756,76 @@ int launch(const Operand& p, const Operand& q, LowpArgs a, cudaStream_t st) {
   return IC_OK;
 }
 
+// block scales as [128-row tile][tile along K][512 bytes]; boxes of `tiles` x `atoms` tiles, zero beyond the matrix
+int make_scale_map(CUtensorMap* tm, const uint8_t* base, int64_t row_tiles, int64_t ktiles, int tiles, int atoms) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(IC_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[3] = {128, (cuuint64_t)ktiles, (cuuint64_t)row_tiles};
+  cuuint64_t strides[2] = {512, (cuuint64_t)ktiles * 512};
+  cuuint32_t box[3] = {128, (cuuint32_t)tiles, (cuuint32_t)atoms};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(tm, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<uint8_t*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(IC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for %lld scale tiles", (int)r, (long long)ktiles);
+  return IC_OK;
+}
+
+template <int KIND>
+int launch_pair(const Operand& p, const Operand& q, LowpArgs a, cudaStream_t st) {
+  using C = PairCfg<KIND>;
+  static std::atomic<unsigned long long> done{0};
+  IC_TRY(once_per_device(done, [] {
+    IC_CUDA(cudaFuncSetAttribute(lowp_pair_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    return (int)IC_OK;
+  }));
+  CUtensorMap tp, tq, tps, tqs;
+  IC_TRY(make_map(&tp, p.codes, p.rows, a.kbytes, p.ld, 128));
+  IC_TRY(make_map(&tq, q.codes, q.rows, a.kbytes, q.ld, 128));
+  if (C::FP4) {
+    IC_TRY(make_scale_map(&tps, p.scales, cdiv(p.rows, 128), a.ktiles, C::SF_TILES, 1));
+    IC_TRY(make_scale_map(&tqs, q.scales, cdiv(q.rows, 128), a.ktiles, C::SF_TILES, 2));
+  } else {
+    tps = tp, tqs = tq;
+  }
+  a.pm = (int)p.rows, a.qn = (int)q.rows;
+  a.p_row = p.row, a.q_row = q.row, a.p_half = p.half, a.q_half = q.half;
+  const int64_t tiles = cdiv(p.rows, 256) * cdiv(q.rows, C::BN);
+  if (tiles > INT32_MAX / 2) return fail(IC_ERR_UNSUPPORTED, "matmul: too many tiles");
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(384, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  // as many pairs as the device holds at once (an odd SM of a GPC has no partner)
+  static std::atomic<int> resident[64];
+  int dev = 0;
+  IC_CUDA(cudaGetDevice(&dev));
+  int pairs = resident[dev & 63].load();
+  if (!pairs) {
+    cfg.gridDim = dim3(2, 1, 1);
+    IC_CUDA(cudaOccupancyMaxActiveClusters(&pairs, lowp_pair_kernel<KIND>, &cfg));
+    if (pairs < 1) return fail(IC_ERR_CUDA, "matmul: no CTA pair fits the device");
+    resident[dev & 63].store(pairs);
+  }
+  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, pairs)), 1, 1);
+  IC_CUDA(cudaLaunchKernelEx(&cfg, lowp_pair_kernel<KIND>, tp, tq, tps, tqs, a));
+  IC_CHECK_LAUNCH();
+  return IC_OK;
+}
+
 // x [m, k] times w [n, k]^T.  Up to 128 activation rows the weights take the
 // 128-row side and the activations a tile as narrow as they are.
 template <int KIND>
 int matmul(const Operand& x, const Operand& w, LowpArgs a, cudaStream_t st) {
   a.swap = x.rows <= 128;
+  if (!a.swap && cdiv(x.rows, 256) * cdiv(w.rows, 256) >= 74) return launch_pair<KIND>(x, w, a, st);
   if (!a.swap) return launch<KIND, 128>(x, w, a, st);
   if (x.rows <= 16) return launch<KIND, 16>(w, x, a, st);
   if (x.rows <= 32) return launch<KIND, 32>(w, x, a, st);

@@ -313,7 +313,8 @@ PRODUCTS = [
     (64, 64, 4096, torch.float32, False), (65, 200, 512, torch.bfloat16, True), (128, 384, 1024, torch.float32, True),
     (129, 128, 320, torch.bfloat16, False), (300, 520, 2080, torch.float32, True), (257, 1024, 4096, torch.bfloat16, True),
     (1, 4096, 16384, torch.bfloat16, False), (1000, 77, 640, torch.float16, False), (5, 3000, 32, torch.float32, False),
-    (2304, 2200, 800, torch.bfloat16, True),
+    (2304, 2200, 800, torch.bfloat16, True), (2400, 2177, 1433, torch.float16, True), (4700, 1300, 320, torch.float32, False),
+    (2305, 2304, 4096, torch.float32, True),
 ]
 
 
