@@ -58,6 +58,9 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, unsigned* flags) {
   return mbar_wait_bounded(bar, parity, flags, WAIT_LIMIT_NS);
 }
@@ -71,6 +74,19 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
+}
+// One lane of a converged warp.  The issuing warps run their loops with all
+// lanes and elect around the instruction: addresses and descriptors then stay
+// in uniform registers (a loop entered by one lane moved each operand of each
+// instruction there, 67 cycles per tcgen05 instruction on B200).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+// every lane waits; true where all of them saw the phase complete (the warp stays converged either way)
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, unsigned* flags) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, flags));
 }
 // K-major operand in 128-byte swizzled rows: 8-row groups 1024 bytes apart
 __device__ __forceinline__ uint64_t operand_desc(uint32_t saddr) {
@@ -161,6 +177,26 @@ __device__ __forceinline__ float load_any(const void* p, int type, long long i) 
   if (type == IC_F32) return static_cast<const float*>(p)[i];
   if (type == IC_F16) return __half2float(static_cast<const __half*>(p)[i]);
   return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+// v[i] = p[first + 32 i], zero beyond `limit` or without p; the loads of all N are in flight together
+template <int N>
+__device__ __forceinline__ void load_strided(const void* p, int type, int first, int limit, float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = 0.f;
+  if (!p) return;
+  if (type == IC_F32) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (first + 32 * i < limit) v[i] = static_cast<const float*>(p)[first + 32 * i];
+  } else if (type == IC_F16) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (first + 32 * i < limit) v[i] = __half2float(static_cast<const __half*>(p)[first + 32 * i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (first + 32 * i < limit) v[i] = __bfloat162float(static_cast<const __nv_bfloat16*>(p)[first + 32 * i]);
+  }
 }
 __device__ __forceinline__ void store_any(void* p, int type, long long i, float v) {
   if (type == IC_F32) static_cast<float*>(p)[i] = v;
@@ -257,40 +293,47 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
     }
     // no copy of this CTA is in flight when it leaves (already true unless a wait gave up)
     for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(full_bar(i % STAGES), (i / STAGES) & 1, a.flags);
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
-    const uint32_t sf0 = tmem + C::ACC_COLS;
+    const uint32_t base0 = smem_u32(smem), sf0 = tmem + C::ACC_COLS;
+    const uint64_t pd = operand_desc(base0), qd = operand_desc(base0 + C::P_BYTES), sd = scale_desc(base0 + C::P_BYTES + C::Q_BYTES);
     const uint32_t qcol = C::FP4 ? (uint32_t)((q0 & 127) >> 5) : 0u;  // narrow tiles start inside a 128-row scale tile
-    for (int i = 0; i < n; ++i) {
-      const int s = i % STAGES;
-      if (!mbar_wait(full_bar(s), (i / STAGES) & 1, a.flags)) break;
+    int s = 0, left = a.kbytes - kt0 * ROW_BYTES;
+    uint32_t ph = 0;
+    for (int i = 0; i < n; ++i, left -= ROW_BYTES) {
+      if (!warp_wait(full_bar(s), ph, a.flags)) break;
       asm volatile("tcgen05.fence::after_thread_sync;");
-      const uint32_t base = smem_u32(smem + s * C::STAGE_BYTES);
-      const int steps = min(4, (a.kbytes - (kt0 + i) * ROW_BYTES + 31) / 32);  // 32 bytes of K each
+      const uint32_t at = (uint32_t)(s * C::STAGE_BYTES) >> 4;  // the descriptors' address field counts 16 bytes
       const uint32_t sfp = sf0 + s * C::SF_COLS, sfq = sfp + C::SF_TILES * 4;
-      if (C::FP4) {
-        const uint32_t ps = base + C::P_BYTES + C::Q_BYTES, qs = ps + C::PS_BYTES;
-        const int tiles = KIND == IC_NVFP4 ? steps : (steps + 1) / 2;
+      const int steps = min(4, (left + 31) >> 5);  // 32 bytes of K each
+      if (elect_one()) {
+        if (C::FP4) {
+          const int tiles = KIND == IC_NVFP4 ? steps : (steps + 1) / 2;
 #pragma unroll
-        for (int t = 0; t < C::SF_TILES; ++t) {
-          if (t >= tiles) break;
-          copy_scales(sfp + t * 4, scale_desc(ps + t * 512));
+          for (int t = 0; t < C::SF_TILES; ++t) {
+            if (t >= tiles) break;
+            copy_scales(sfp + t * 4, sd + at + t * 32);
 #pragma unroll
-          for (int u = 0; u < C::Q_ATOMS; ++u)
-            copy_scales(sfq + (t * C::Q_ATOMS + u) * 4, scale_desc(qs + u * C::PS_BYTES + t * 512));
+            for (int u = 0; u < C::Q_ATOMS; ++u)
+              copy_scales(sfq + (t * C::Q_ATOMS + u) * 4, sd + at + ((u + 1) * C::PS_BYTES >> 4) + t * 32);
+          }
         }
-      }
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        if (kk >= steps) break;
-        const int t = KIND == IC_NVFP4 ? kk : kk >> 1;
-        const uint32_t id = KIND == IC_MXFP4 && (kk & 1) ? C::IDESC | (2u << 4) | (2u << 29) : C::IDESC;
-        mma<KIND>(tmem, operand_desc(base + kk * 32), operand_desc(base + C::P_BYTES + kk * 32), id, sfp + t * 4,
-                  sfq + t * C::Q_ATOMS * 4 + qcol, (i | kk) ? 1u : 0u);
+        for (int kk = 0; kk < 4; ++kk) {
+          if (kk >= steps) break;
+          const int t = KIND == IC_NVFP4 ? kk : kk >> 1;
+          const uint32_t id = KIND == IC_MXFP4 && (kk & 1) ? C::IDESC | (2u << 4) | (2u << 29) : C::IDESC;
+          mma<KIND>(tmem, pd + at + kk * 2, qd + at + kk * 2, id, sfp + t * 4, sfq + t * C::Q_ATOMS * 4 + qcol, (i | kk) ? 1u : 0u);
+        }
+        mma_commit(empty_bar(s));
+        if (i == n - 1) mma_commit(acc_bar);
       }
-      mma_commit(empty_bar(s));
+      __syncwarp();
+      if (++s == STAGES) {
+        s = 0;
+        ph ^= 1;
+      }
     }
-    mma_commit(acc_bar);
   }
   __syncwarp();
 
@@ -365,6 +408,12 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
 //   empty[s] in each CTA: the commit of the products that read the stage
 //   accf     in each CTA: the commit of a tile's last product
 //   acce     leader only: 16 epilogue warps have taken the accumulator
+// What the epilogue applies to one 128 x 256 part of a tile
+struct Factors {
+  float col[256], bias[256], row[128];
+  int zp[256], sum[128];
+};
+
 constexpr int PAIR_GROUP = 8;  // 256-row tiles per group of the tile order
 
 template <int KIND>
@@ -375,12 +424,11 @@ struct PairCfg {
   static constexpr int P_BYTES = 128 * ROW_BYTES, Q_BYTES = 128 * ROW_BYTES;
   static constexpr int PS_BYTES = SF_TILES * 512, QS_BYTES = 2 * PS_BYTES;
   static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES + PS_BYTES + QS_BYTES;
-  static constexpr int STAGES = 4;
+  static constexpr int STAGES = FP4 ? 5 : 6;
   static constexpr int SF_COLS = SF_TILES * 12;
   static constexpr int TMEM_COLS = 512;
-  static constexpr int OUT_BYTES = 8 * 4096;      // per epilogue warp: 32 rows of 128 bytes
-  static constexpr int FACTOR_BYTES = 8 * 1024;   // per epilogue warp: 128 column factors and biases
-  static constexpr int SMEM = STAGES * STAGE_BYTES + OUT_BYTES + FACTOR_BYTES + 1024 + 256;
+  static constexpr int OUT_BYTES = 8 * 2048;  // per epilogue warp: 32 rows of 64 bytes
+  static constexpr int SMEM = STAGES * STAGE_BYTES + OUT_BYTES + 2 * (int)sizeof(Factors) + 1024 + 256;
   static_assert(BN + STAGES * SF_COLS <= TMEM_COLS, "tensor memory");
   static_assert(SMEM <= 232448, "shared memory");
   static constexpr uint32_t IDESC =
@@ -455,53 +503,92 @@ __device__ __forceinline__ void remote_arrive(uint32_t cluster_addr) {
         "=r"((r)[30]), "=r"((r)[31])                                                             \
       : "r"(taddr))
 
-// One warp's 32 rows x 128 columns of finished sums to y.  `out` is the warp's
-// 4 KB of shared memory: rows of 128 bytes, 16-byte pieces XOR-swizzled by the
-// row, written one row per lane and read back eight lanes to a row, so that
-// global stores cover whole 128-byte lines.
+// One lane's row of four sums from column c of the tile, scaled
+template <int KIND>
+__device__ __forceinline__ void finish4(const LowpArgs& a, const uint32_t* acc, const Factors& f, int c, float rowf, int sum,
+                                        float (&v)[4]) {
+  float s[4] = {1.f, 1.f, 1.f, 1.f}, b[4];
+  if (KIND != IC_MXFP4) *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(f.col + c);
+  if (a.bias) *reinterpret_cast<float4*>(b) = *reinterpret_cast<const float4*>(f.bias + c);
+  int z[4];
+  if (KIND == IC_INT8 && a.zp) *reinterpret_cast<int4*>(z) = *reinterpret_cast<const int4*>(f.zp + c);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    if (KIND == IC_INT8) v[u] = (float)((int)acc[u] - (a.zp ? z[u] * sum : 0));
+    else v[u] = __uint_as_float(acc[u]);
+    if (KIND != IC_MXFP4) v[u] = __fmul_rn(__fmul_rn(v[u], rowf), s[u]);
+    if (a.bias) v[u] = __fadd_rn(v[u], b[u]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ T to_out(float v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
+  else return __float2bfloat16_rn(v);
+}
+
+// One warp's 32 rows x 128 columns of sums, from column c0 of the tile, to y.
+// Rows that are 32-byte aligned: each lane stores its own row in whole 32-byte
+// sectors, past shared memory, whose bandwidth the loads and products of the
+// next tile take up.  Other rows: through the warp's 2 KB `out`, 64 bytes of
+// each row at a time, so that neighbouring lanes store neighbouring elements.
 template <int KIND, typename T>
 __device__ __forceinline__ void store_block(const LowpArgs& a, const uint32_t (&acc)[128], unsigned char* out,
-                                            const float* factor, const float* bias, float rowf, int row0,
-                                            int col0, int lane) {
-  constexpr int G = 128 / sizeof(T);  // columns per pass
-  constexpr int V = 16 / sizeof(T);
+                                            const Factors& f, int r0, int c0, int row0, int col0, int lane) {
   T* y = static_cast<T*>(a.y);
-  const bool vec = (reinterpret_cast<uintptr_t>(y) & 15) == 0 && (a.ldy * (long long)sizeof(T)) % 16 == 0;
+  const float rowf = f.row[r0 + lane];
+  const int sum = f.sum[r0 + lane];
+  if (((reinterpret_cast<uintptr_t>(y) | (uintptr_t)(a.ldy * (long long)sizeof(T))) & 31) == 0) {
+    constexpr int V = 32 / sizeof(T);
+    T* to = y + (long long)(row0 + lane) * a.ldy + col0;
+    const int left = row0 + lane < a.pm ? a.qn - col0 : 0;
+#pragma unroll
+    for (int c = 0; c < 128; c += V) {
+      alignas(32) T e[V];
+#pragma unroll
+      for (int u = 0; u < V; u += 4) {
+        float v[4];
+        finish4<KIND>(a, acc + c + u, f, c0 + c + u, rowf, sum, v);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) e[u + w] = to_out<T>(v[w]);
+      }
+      if (c + V <= left) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(e);
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + c), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                     "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                     : "memory");
+      } else {
+#pragma unroll
+        for (int u = 0; u < V; ++u)
+          if (c + u < left) to[c + u] = e[u];
+      }
+    }
+    return;
+  }
+  constexpr int G = 64 / sizeof(T);  // columns per pass
+  constexpr int V = 16 / sizeof(T);
 #pragma unroll
   for (int g = 0; g < 128 / G; ++g) {
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-      uint4 piece;
-      T* e = reinterpret_cast<T*>(&piece);
+    for (int p = 0; p < 4; ++p) {
+      alignas(16) T e[V];
 #pragma unroll
-      for (int u = 0; u < V; ++u) {
+      for (int u = 0; u < V; u += 4) {
         const int c = g * G + p * V + u;
-        float v;
-        if (KIND == IC_INT8) v = (float)(int)acc[c];
-        else v = __uint_as_float(acc[c]);
-        if (KIND != IC_MXFP4) v = __fmul_rn(__fmul_rn(v, rowf), factor[c]);
-        if (a.bias) v = __fadd_rn(v, bias[c]);
-        if constexpr (sizeof(T) == 4) e[u] = v;
-        else if constexpr (std::is_same<T, __half>::value) e[u] = __float2half_rn(v);
-        else e[u] = __float2bfloat16_rn(v);
+        float v[4];
+        finish4<KIND>(a, acc + c, f, c0 + c, rowf, sum, v);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) e[u + w] = to_out<T>(v[w]);
       }
-      *reinterpret_cast<uint4*>(out + lane * 128 + ((p ^ (lane & 7)) << 4)) = piece;
+      *reinterpret_cast<uint4*>(out + lane * 64 + ((p ^ ((lane >> 1) & 3)) << 4)) = *reinterpret_cast<const uint4*>(e);
     }
     __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = i * 4 + (lane >> 3), p = lane & 7;
-      const uint4 piece = *reinterpret_cast<const uint4*>(out + r * 128 + ((p ^ (r & 7)) << 4));
-      const int col = col0 + g * G + p * V;
-      if (row0 + r < a.pm && col < a.qn) {
-        T* to = y + (long long)(row0 + r) * a.ldy + col;
-        if (vec && col + V <= a.qn) {
-          *reinterpret_cast<uint4*>(to) = piece;
-        } else {
-          const T* e = reinterpret_cast<const T*>(&piece);
-          for (int u = 0; u < V && col + u < a.qn; ++u) to[u] = e[u];
-        }
-      }
+    const int rows = min(32, a.pm - row0), cols = min(G, a.qn - col0 - g * G);
+    for (int i = lane; i < rows * G; i += 32) {
+      const int r = i / G, c = i % G;
+      if (c < cols)
+        y[(long long)(row0 + r) * a.ldy + col0 + g * G + c] =
+            *reinterpret_cast<const T*>(out + r * 64 + (((c / V) ^ ((r >> 1) & 3)) << 4) + (c % V) * sizeof(T));
     }
     __syncwarp();
   }
@@ -516,12 +603,14 @@ __global__ void __launch_bounds__(384, 1)
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* out_smem = smem + STAGES * C::STAGE_BYTES;
-  float* factor_smem = reinterpret_cast<float*>(out_smem + C::OUT_BYTES);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(out_smem + C::OUT_BYTES + C::FACTOR_BYTES);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 2);
+  Factors* factors = reinterpret_cast<Factors*>(out_smem + C::OUT_BYTES);  // two, by turns
+  uint64_t* bars = reinterpret_cast<uint64_t*>(out_smem + C::OUT_BYTES + 2 * sizeof(Factors));
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
   auto full_bar = [&](int s) { return smem_u32(bars + s); };
   auto empty_bar = [&](int s) { return smem_u32(bars + STAGES + s); };
   const uint32_t accf = smem_u32(bars + 2 * STAGES), acce = smem_u32(bars + 2 * STAGES + 1);
+  auto facf = [&](int b) { return smem_u32(bars + 2 * STAGES + 2 + b); };
+  auto face = [&](int b) { return smem_u32(bars + 2 * STAGES + 4 + b); };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -543,6 +632,10 @@ __global__ void __launch_bounds__(384, 1)
     }
     mbar_init(accf, 1);
     mbar_init(acce, 16);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(facf(b), 32);
+      mbar_init(face(b), 8);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
@@ -584,64 +677,102 @@ __global__ void __launch_bounds__(384, 1)
     // no copy is in flight when the pair leaves (already true unless a wait gave up)
     if (leader)
       for (int i = max(0, g - STAGES); i < g; ++i) mbar_wait(full_bar(i % STAGES), (i / STAGES) & 1, a.flags);
-  } else if (warp == 1 && lane == 0 && leader) {
+  } else if (warp == 1 && leader) {
     // ---------------- MMA issuer (leader) ----------------
-    int g = 0, t = 0;
+    const uint32_t base0 = smem_u32(smem);
+    const uint64_t pd = operand_desc(base0), qd = operand_desc(base0 + C::P_BYTES), sd = scale_desc(base0 + C::P_BYTES + C::Q_BYTES);
+    int s = 0, t = 0;
+    uint32_t ph = 0;
     bool ok = true;
     for (int tile = pair; tile < tiles && ok; tile += pairs, ++t) {
-      if (t > 0 && !mbar_wait(acce, (t & 1) ^ 1, a.flags)) break;
+      if (t > 0 && !warp_wait(acce, (t & 1) ^ 1, a.flags)) break;
       asm volatile("tcgen05.fence::after_thread_sync;");
-      for (int i = 0; i < n; ++i, ++g) {
-        const int s = g % STAGES;
-        if (!mbar_wait(full_bar(s), (g / STAGES) & 1, a.flags)) {
+      int left = a.kbytes;
+      for (int i = 0; i < n; ++i, left -= ROW_BYTES) {
+        if (!warp_wait(full_bar(s), ph, a.flags)) {
           ok = false;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;");
-        const uint32_t base = smem_u32(smem + s * C::STAGE_BYTES);
-        const int steps = min(4, (a.kbytes - i * ROW_BYTES + 31) / 32);
+        const uint32_t at = (uint32_t)(s * C::STAGE_BYTES) >> 4;  // the descriptors' address field counts 16 bytes
         const uint32_t sfp = tmem + C::BN + s * C::SF_COLS, sfq = sfp + C::SF_TILES * 4;
-        if (C::FP4) {
-          const uint32_t ps = base + C::P_BYTES + C::Q_BYTES, qs = ps + C::PS_BYTES;
+        const int steps = min(4, (left + 31) >> 5);
+        if (elect_one()) {
+          if (C::FP4) {
 #pragma unroll
-          for (int k = 0; k < C::SF_TILES; ++k) {
-            copy_scales_pair(sfp + k * 4, scale_desc(ps + k * 512));
-            copy_scales_pair(sfq + k * 8, scale_desc(qs + k * 512));
-            copy_scales_pair(sfq + k * 8 + 4, scale_desc(qs + C::PS_BYTES + k * 512));
+            for (int k = 0; k < C::SF_TILES; ++k) {
+              copy_scales_pair(sfp + k * 4, sd + at + k * 32);
+              copy_scales_pair(sfq + k * 8, sd + at + (C::PS_BYTES >> 4) + k * 32);
+              copy_scales_pair(sfq + k * 8 + 4, sd + at + (2 * C::PS_BYTES >> 4) + k * 32);
+            }
           }
-        }
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          if (kk >= steps) break;
-          const int k = KIND == IC_NVFP4 ? kk : kk >> 1;
-          const uint32_t id = KIND == IC_MXFP4 && (kk & 1) ? C::IDESC | (2u << 4) | (2u << 29) : C::IDESC;
-          mma_pair<KIND>(tmem, operand_desc(base + kk * 32), operand_desc(base + C::P_BYTES + kk * 32), id, sfp + k * 4,
-                         sfq + k * 8, (i | kk) ? 1u : 0u);
+          for (int kk = 0; kk < 4; ++kk) {
+            if (kk >= steps) break;
+            const int k = KIND == IC_NVFP4 ? kk : kk >> 1;
+            const uint32_t id = KIND == IC_MXFP4 && (kk & 1) ? C::IDESC | (2u << 4) | (2u << 29) : C::IDESC;
+            mma_pair<KIND>(tmem, pd + at + kk * 2, qd + at + kk * 2, id, sfp + k * 4, sfq + k * 8, (i | kk) ? 1u : 0u);
+          }
+          mma_commit_pair(empty_bar(s));
+          if (i == n - 1) mma_commit_pair(accf);
         }
-        mma_commit_pair(empty_bar(s));
+        __syncwarp();
+        if (++s == STAGES) {
+          s = 0;
+          ph ^= 1;
+        }
       }
-      mma_commit_pair(accf);
     }
-  } else if (warp >= 4) {
-    // ---------------- epilogue (both CTAs, own rows) ----------------
-    const int q = warp & 3, h = (warp - 4) >> 2, ew = warp - 4;
-    unsigned char* out = out_smem + ew * 4096;
-    float* factor = factor_smem + ew * 256;  // [128] factors, [128] biases
+  } else if (warp == 3) {
+    // ---------------- factors of the coming tile (both CTAs) ----------------
     int t = 0;
     for (int tile = pair; tile < tiles; tile += pairs, ++t) {
       int p0, q0;
       place(tile, p0, q0);
-      const int row0 = p0 + (int)rank * 128 + q * 32, row = row0 + lane, col0 = q0 + h * 128;
+      Factors& f = factors[t & 1];
+      if (t >= 2 && !warp_wait(face(t & 1), ((t >> 1) & 1) ^ 1, a.flags)) break;
+      const int row0 = p0 + (int)rank * 128;
+      float cf[8], cb[8], rf[4];
+      load_strided(a.q_row, a.q_half ? IC_F16 : IC_F32, q0 + lane, a.qn, cf);
+      load_strided(a.bias, a.bias_type, q0 + lane, a.qn, cb);
+      load_strided(a.p_row, a.p_half ? IC_F16 : IC_F32, row0 + lane, a.pm, rf);
+      int zp[8], sum[4];
+      if (KIND == IC_INT8 && a.zp) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) zp[i] = q0 + i * 32 + lane < a.qn ? a.zp[q0 + i * 32 + lane] : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = row0 + i * 32 + lane < a.pm ? a.sums[row0 + i * 32 + lane] : 0;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) zp[i] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f.col[i * 32 + lane] = cf[i];
+        f.bias[i * 32 + lane] = cb[i];
+        f.zp[i * 32 + lane] = zp[i];
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int c = i * 32 + lane, col = col0 + c;
-        factor[c] = a.q_row && col < a.qn ? load_any(a.q_row, a.q_half ? IC_F16 : IC_F32, col) : 0.f;
-        factor[128 + c] = a.bias && col < a.qn ? load_any(a.bias, a.bias_type, col) : 0.f;
+        f.row[i * 32 + lane] = rf[i];
+        f.sum[i * 32 + lane] = sum[i];
       }
-      const float rowf = a.p_row && row < a.pm ? load_any(a.p_row, a.p_half ? IC_F16 : IC_F32, row) : 0.f;
-      __syncwarp();
-      bool ok = mbar_wait(accf, t & 1, a.flags);
-      if (!ok) mbar_wait(accf, t & 1, a.flags);  // products in flight end before their tensor memory is freed
+      mbar_arrive(facf(t & 1));
+    }
+  } else if (warp >= 4) {
+    // ---------------- epilogue (both CTAs, own rows) ----------------
+    const int q = warp & 3, h = (warp - 4) >> 2;
+    unsigned char* out = out_smem + (warp - 4) * 2048;
+    int t = 0;
+    for (int tile = pair; tile < tiles; tile += pairs, ++t) {
+      int p0, q0;
+      place(tile, p0, q0);
+      const int row0 = p0 + (int)rank * 128 + q * 32, col0 = q0 + h * 128;
+      bool ok = warp_wait(facf(t & 1), (t >> 1) & 1, a.flags);
+      ok &= warp_wait(accf, t & 1, a.flags);
+      if (!ok) warp_wait(accf, t & 1, a.flags);  // products in flight end before their tensor memory is freed
       asm volatile("tcgen05.fence::after_thread_sync;");
       uint32_t acc[128];
       const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * 128);
@@ -652,18 +783,12 @@ __global__ void __launch_bounds__(384, 1)
       __syncwarp();
       if (lane == 0) remote_arrive(map_to_rank(acce, 0));
       if (!ok) break;
-      if (KIND == IC_INT8 && a.zp) {
-        const int sum = row < a.pm ? a.sums[row] : 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int col = col0 + i * 32 + lane, z = col < a.qn ? a.zp[col] : 0;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) acc[i * 32 + j] -= (uint32_t)(__shfl_sync(0xffffffffu, z, j) * sum);
-        }
-      }
-      if (a.out_type == IC_BF16) store_block<KIND, __nv_bfloat16>(a, acc, out, factor, factor + 128, rowf, row0, col0, lane);
-      else if (a.out_type == IC_F16) store_block<KIND, __half>(a, acc, out, factor, factor + 128, rowf, row0, col0, lane);
-      else store_block<KIND, float>(a, acc, out, factor, factor + 128, rowf, row0, col0, lane);
+      const Factors& f = factors[t & 1];
+      if (a.out_type == IC_BF16) store_block<KIND, __nv_bfloat16>(a, acc, out, f, q * 32, h * 128, row0, col0, lane);
+      else if (a.out_type == IC_F16) store_block<KIND, __half>(a, acc, out, f, q * 32, h * 128, row0, col0, lane);
+      else store_block<KIND, float>(a, acc, out, f, q * 32, h * 128, row0, col0, lane);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(face(t & 1));  // every lane has read the factors
     }
   }
   __syncwarp();
