@@ -400,14 +400,17 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
 // and of Q and the scales of its P rows and of all Q rows.  Per SM and 128
 // bytes of K that is 32 KB of operands for 512 tensor-core cycles; a single
 // CTA's 128 x 128 tile needs 32 KB for 256, more than L2 delivers.
-// The accumulator takes 256 of the 512 TMEM columns and the scales most of the
-// rest, so it is not doubled: eight epilogue warps move it to registers at
-// once (128 columns each), release it, and scale, convert and store while the
-// next tile's products run.
+// Tensor memory: INT8 has two accumulators of 256 columns, by turns.  The 4-bit
+// kinds have one and every stage's scales (overlapping two accumulators left
+// room for the scales of three stages: 127 instead of 117 us at
+// 4608 x 4096 x 16384 nvfp4).  Eight epilogue warps move an accumulator to
+// registers at once and release it; scaling, conversion and stores run under
+// the next products.
 //   full[s]  leader only: the bytes of both CTAs' loads
 //   empty[s] in each CTA: the commit of the products that read the stage
-//   accf     in each CTA: the commit of a tile's last product
-//   acce     leader only: 16 epilogue warps have taken the accumulator
+//   accf[b]  in each CTA: the commit of a tile's last product into accumulator b
+//   acce[b]  leader only: 16 epilogue warps have taken accumulator b
+//   facf/face[b] in each CTA: the tile's factors are loaded / have been read
 // What the epilogue applies to one 128 x 256 part of a tile
 struct Factors {
   float col[256], bias[256], row[128];
@@ -426,10 +429,11 @@ struct PairCfg {
   static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES + PS_BYTES + QS_BYTES;
   static constexpr int STAGES = FP4 ? 5 : 6;
   static constexpr int SF_COLS = SF_TILES * 12;
+  static constexpr int NACC = FP4 ? 1 : 2;
   static constexpr int TMEM_COLS = 512;
   static constexpr int OUT_BYTES = 8 * 2048;  // per epilogue warp: 32 rows of 64 bytes
   static constexpr int SMEM = STAGES * STAGE_BYTES + OUT_BYTES + 2 * (int)sizeof(Factors) + 1024 + 256;
-  static_assert(BN + STAGES * SF_COLS <= TMEM_COLS, "tensor memory");
+  static_assert(NACC * BN + STAGES * SF_COLS <= TMEM_COLS, "tensor memory");
   static_assert(SMEM <= 232448, "shared memory");
   static constexpr uint32_t IDESC =
       KIND == IC_INT8 ? (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(256 >> 4) << 24)
@@ -605,12 +609,13 @@ __global__ void __launch_bounds__(384, 1)
   unsigned char* out_smem = smem + STAGES * C::STAGE_BYTES;
   Factors* factors = reinterpret_cast<Factors*>(out_smem + C::OUT_BYTES);  // two, by turns
   uint64_t* bars = reinterpret_cast<uint64_t*>(out_smem + C::OUT_BYTES + 2 * sizeof(Factors));
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 8);
   auto full_bar = [&](int s) { return smem_u32(bars + s); };
   auto empty_bar = [&](int s) { return smem_u32(bars + STAGES + s); };
-  const uint32_t accf = smem_u32(bars + 2 * STAGES), acce = smem_u32(bars + 2 * STAGES + 1);
-  auto facf = [&](int b) { return smem_u32(bars + 2 * STAGES + 2 + b); };
-  auto face = [&](int b) { return smem_u32(bars + 2 * STAGES + 4 + b); };
+  auto accf = [&](int b) { return smem_u32(bars + 2 * STAGES + b); };
+  auto acce = [&](int b) { return smem_u32(bars + 2 * STAGES + 2 + b); };
+  auto facf = [&](int b) { return smem_u32(bars + 2 * STAGES + 4 + b); };
+  auto face = [&](int b) { return smem_u32(bars + 2 * STAGES + 6 + b); };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -630,9 +635,9 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
     }
-    mbar_init(accf, 1);
-    mbar_init(acce, 16);
     for (int b = 0; b < 2; ++b) {
+      mbar_init(accf(b), 1);
+      mbar_init(acce(b), 16);
       mbar_init(facf(b), 32);
       mbar_init(face(b), 8);
     }
@@ -685,7 +690,9 @@ __global__ void __launch_bounds__(384, 1)
     uint32_t ph = 0;
     bool ok = true;
     for (int tile = pair; tile < tiles && ok; tile += pairs, ++t) {
-      if (t > 0 && !warp_wait(acce, (t & 1) ^ 1, a.flags)) break;
+      const int b = t % C::NACC;
+      if (t >= C::NACC && !warp_wait(acce(b), ((t / C::NACC) & 1) ^ 1, a.flags)) break;
+      const uint32_t acc = tmem + b * C::BN;
       asm volatile("tcgen05.fence::after_thread_sync;");
       int left = a.kbytes;
       for (int i = 0; i < n; ++i, left -= ROW_BYTES) {
@@ -711,10 +718,10 @@ __global__ void __launch_bounds__(384, 1)
             if (kk >= steps) break;
             const int k = KIND == IC_NVFP4 ? kk : kk >> 1;
             const uint32_t id = KIND == IC_MXFP4 && (kk & 1) ? C::IDESC | (2u << 4) | (2u << 29) : C::IDESC;
-            mma_pair<KIND>(tmem, pd + at + kk * 2, qd + at + kk * 2, id, sfp + k * 4, sfq + k * 8, (i | kk) ? 1u : 0u);
+            mma_pair<KIND>(acc, pd + at + kk * 2, qd + at + kk * 2, id, sfp + k * 4, sfq + k * 8, (i | kk) ? 1u : 0u);
           }
           mma_commit_pair(empty_bar(s));
-          if (i == n - 1) mma_commit_pair(accf);
+          if (i == n - 1) mma_commit_pair(accf(b));
         }
         __syncwarp();
         if (++s == STAGES) {
@@ -771,17 +778,18 @@ __global__ void __launch_bounds__(384, 1)
       place(tile, p0, q0);
       const int row0 = p0 + (int)rank * 128 + q * 32, col0 = q0 + h * 128;
       bool ok = warp_wait(facf(t & 1), (t >> 1) & 1, a.flags);
-      ok &= warp_wait(accf, t & 1, a.flags);
-      if (!ok) warp_wait(accf, t & 1, a.flags);  // products in flight end before their tensor memory is freed
+      const int b = t % C::NACC;
+      ok &= warp_wait(accf(b), (t / C::NACC) & 1, a.flags);
+      if (!ok) warp_wait(accf(b), (t / C::NACC) & 1, a.flags);  // products in flight end before their tensor memory is freed
       asm volatile("tcgen05.fence::after_thread_sync;");
       uint32_t acc[128];
-      const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * 128);
+      const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * C::BN + h * 128);
 #pragma unroll
       for (int i = 0; i < 4; ++i) IC_TMEM_LD32(at + i * 32, acc + i * 32);
       asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;");
       __syncwarp();
-      if (lane == 0) remote_arrive(map_to_rank(acce, 0));
+      if (lane == 0) remote_arrive(map_to_rank(acce(b), 0));
       if (!ok) break;
       const Factors& f = factors[t & 1];
       if (a.out_type == IC_BF16) store_block<KIND, __nv_bfloat16>(a, acc, out, f, q * 32, h * 128, row0, col0, lane);
