@@ -2,8 +2,6 @@
 
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _native as nat
@@ -48,6 +46,13 @@ def workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
 
 
-def on(dev: torch.device):
-    """Context in which ``dev`` is the current device (nothing to enter when it already is)."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def call(name: str, dev: torch.device, *args) -> None:
+    """Run entry point ``name`` on ``dev``'s current stream (its last argument) with ``dev`` current."""
+    fn = getattr(nat.load(), name)
+    if dev.index == torch.cuda.current_device():
+        status = fn(*args, nat.stream_ptr(dev))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, nat.stream_ptr(dev))
+    if status:
+        nat.check(status, name[3:])

@@ -141,13 +141,9 @@ class _Checked:
         self._lib = lib
         self._fns = {}
         for name, (_, args) in SIGNATURES.items():
-            fn, n = getattr(lib, name), len(args)
-
-            def call(*a, _fn=fn, _n=n, _name=name):
-                if len(a) != _n:
-                    raise TypeError(f"{_name} takes {_n} arguments, got {len(a)}")
-                return _fn(*a)
-            self._fns[name] = call
+            # a function of exactly the declared arguments: Python itself refuses any other number
+            names = ", ".join(f"a{i}" for i in range(len(args)))
+            self._fns[name] = eval(f"lambda {names}: fn({names})", {"fn": getattr(lib, name)})
 
     def __getattr__(self, name):
         fns = self.__dict__.get("_fns", {})
@@ -183,6 +179,8 @@ _device_ok: dict[int, bool] = {}
 
 def require_device(device: torch.device | None = None) -> torch.device:
     """The CUDA device the kernels run on; raises if there is no sm_100 GPU."""
+    if device is not None and device.type == "cuda" and device.index in _device_ok:
+        return device
     if not torch.cuda.is_available():
         raise RuntimeError("int_crush_converter_b200 needs a CUDA sm_100a (B200) device; none is available")
     if device is None or device.type != "cuda":
@@ -196,7 +194,10 @@ def require_device(device: torch.device | None = None) -> torch.device:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    if index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(index)  # the same stream without building a Stream object
 
 
 def ptr(t):

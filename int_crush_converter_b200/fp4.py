@@ -17,7 +17,7 @@ import dataclasses
 import torch
 
 from . import _native as nat
-from ._dev import back, device_of, on
+from ._dev import back, call, device_of
 from .rotation import _DT, _is_power_of_two, _rotate_rows
 
 FORMATS = {"mxfp4": nat.IC_MXFP4, "nvfp4": nat.IC_NVFP4}
@@ -73,37 +73,38 @@ class FP4Tensor:
 
     def check(self, what: str) -> None:
         """ValueError unless the parts have the types and sizes the kernels read."""
-        if self.fmt not in FORMATS:
-            raise ValueError(f"{what}: fmt must be one of {sorted(FORMATS)}, got {self.fmt!r}")
         p, s, g = self.packed, self.scales, self.row_scale
-        if p.dim() != 2 or p.dtype != torch.uint8 or s.dtype != torch.uint8:
+        block = BLOCK.get(self.fmt)
+        if block is None:
+            raise ValueError(f"{what}: fmt must be one of {sorted(FORMATS)}, got {self.fmt!r}")
+        if p.dim() != 2 or p.dtype is not torch.uint8 or s.dtype is not torch.uint8:
             raise ValueError(f"{what}: packed must be uint8 [rows, columns/2] and scales uint8")
-        rows, kp = p.shape[0], p.shape[1] * 2
-        if kp % 32:
-            raise ValueError(f"{what}: the number of columns must be a multiple of 32, got {kp}")
-        tiles = -(-rows // 128) * _ktiles(self.fmt, kp)
-        if s.numel() != tiles * 512:
-            raise ValueError(f"{what}: {rows} rows of {kp} {self.fmt} columns have {tiles * 512} scale bytes, got {s.numel()}")
-        if (g is None) != (self.fmt == "mxfp4"):
-            raise ValueError(f"{what}: nvfp4 has row scales and mxfp4 none")
-        if g is not None and (g.dtype != torch.float32 or g.numel() != rows or g.device != p.device):
-            raise ValueError(f"{what}: row_scale must be fp32 [rows] on the codes' device")
-        if s.device != p.device:
+        rows, half = p.shape
+        if half & 15:
+            raise ValueError(f"{what}: the number of columns must be a multiple of 32, got {2 * half}")
+        need = -(-rows // 128) * -(-half // (2 * block)) * 512
+        if s.numel() != need:
+            raise ValueError(f"{what}: {rows} rows of {2 * half} {self.fmt} columns have {need} scale bytes, got {s.numel()}")
+        device = p.device
+        if s.device != device:
             raise ValueError(f"{what}: packed and scales must be on one device")
+        if (g is None) != (block == 32):
+            raise ValueError(f"{what}: nvfp4 has row scales and mxfp4 none")
+        if g is not None and (g.dtype is not torch.float32 or g.numel() != rows or g.device != device):
+            raise ValueError(f"{what}: row_scale must be fp32 [rows] on the codes' device")
         if not p.is_contiguous() or not s.is_contiguous() or (g is not None and not g.is_contiguous()):
             raise ValueError(f"{what}: packed, scales and row_scale must be contiguous")
         if (p.data_ptr() | s.data_ptr()) & 15:
             raise ValueError(f"{what}: packed and scales must be 16-byte aligned")
 
-    def lead_shape(self) -> tuple:
-        return (self.rows,) if self.lead is None else tuple(self.lead)
 
-
-def empty_fp4(rows: int, columns: int, fmt: str, dev: torch.device, **kw) -> FP4Tensor:
+def empty_fp4(rows: int, columns: int, fmt: str, dev: torch.device, in_features: int | None = None, rot_size: int = 0,
+              lead: tuple | None = None) -> FP4Tensor:
     """An FP4Tensor of uninitialised parts."""
-    return FP4Tensor(torch.empty(rows, columns // 2, dtype=torch.uint8, device=dev),
-                     torch.empty(-(-rows // 128), _ktiles(fmt, columns), 32, 4, 4, dtype=torch.uint8, device=dev),
-                     torch.empty(rows, dtype=torch.float32, device=dev) if fmt == "nvfp4" else None, fmt, **kw)
+    return FP4Tensor(torch.empty((rows, columns // 2), dtype=torch.uint8, device=dev),
+                     torch.empty((-(-rows // 128), _ktiles(fmt, columns), 32, 4, 4), dtype=torch.uint8, device=dev),
+                     torch.empty((rows,), dtype=torch.float32, device=dev) if fmt == "nvfp4" else None, fmt, in_features,
+                     rot_size, lead)
 
 
 def padded_columns(k: int, fmt: str, rot_size: int) -> int:
@@ -114,10 +115,15 @@ def padded_columns(k: int, fmt: str, rot_size: int) -> int:
 
 def as_rows(x: torch.Tensor, dev: torch.device) -> torch.Tensor:
     """[..., K] -> 2-D rows on ``dev`` with unit column stride (a view where possible)."""
-    x2 = x.to(dev).reshape(-1, x.shape[-1]) if x.dim() != 2 else x.to(dev)
-    if x2.shape[0] and x2.shape[1] and (x2.stride(1) != 1 or x2.stride(0) < x2.shape[1]):
-        x2 = x2.contiguous()
-    return x2
+    if not x.is_cuda:
+        x = x.to(dev)
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    if not x.is_contiguous() and x.numel():
+        pitch_, step = x.stride()
+        if step != 1 or pitch_ < x.shape[1]:
+            x = x.contiguous()
+    return x
 
 
 def pitch(x2: torch.Tensor) -> int:
@@ -145,7 +151,7 @@ def quantize_fp4(x: torch.Tensor, fmt: str = "mxfp4", rot_size: int = 0,
     if row_scale is not None and fmt != "nvfp4":
         raise ValueError("row_scale is for nvfp4")
     dev = device_of(x)
-    lead, k = tuple(x.shape[:-1]), x.shape[-1]
+    lead, k = x.shape[:-1], x.shape[-1]
     x2 = as_rows(x, dev)
     rows, rot = x2.shape[0], rot_size
     stride = 0
@@ -154,16 +160,15 @@ def quantize_fp4(x: torch.Tensor, fmt: str = "mxfp4", rot_size: int = 0,
         if row_scale.numel() not in (1, rows):
             raise ValueError(f"row_scale must have 1 or {rows} values, got {row_scale.numel()}")
         stride = int(row_scale.numel() == rows and rows > 1)
-    with on(dev):
-        if rot and not 16 <= rot <= 512:
+    if rot and not 16 <= rot <= 512:
+        with torch.cuda.device(dev):
             x2 = _rotate_rows(x2, rot, dev) if rows else x2.new_empty(0, padded_columns(k, "int8", rot))
-            rot = 0
-        out = empty_fp4(rows, padded_columns(x2.shape[1], fmt, rot), fmt, dev, in_features=k, rot_size=rot_size, lead=lead)
-        if rows:
-            nat.check(nat.load().ic_fp4_quantize(
-                x2.data_ptr(), _DT[x2.dtype], rows, x2.shape[1], pitch(x2), FORMATS[fmt], rot, out.columns,
-                nat.ptr(row_scale), stride, out.packed.data_ptr(), out.scales.data_ptr(), nat.ptr(out.row_scale),
-                nat.stream_ptr(dev)), "quantize_fp4")
+        rot = 0
+    columns = padded_columns(x2.shape[1], fmt, rot)
+    out = empty_fp4(rows, columns, fmt, dev, k, rot_size, lead)
+    if rows:
+        call("ic_fp4_quantize", dev, x2.data_ptr(), _DT[x2.dtype], rows, x2.shape[1], pitch(x2), FORMATS[fmt], rot, columns,
+             nat.ptr(row_scale), stride, out.packed.data_ptr(), out.scales.data_ptr(), nat.ptr(out.row_scale))
     return out if x.is_cuda else out.to(x.device)
 
 
@@ -173,14 +178,15 @@ def dequantize_fp4(q: FP4Tensor, dtype: torch.dtype = torch.float32) -> torch.Te
     if dtype not in _DT:
         raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     dev = device_of(q.packed)
-    d = q.to(dev)
-    out = torch.empty(d.rows, d.columns, dtype=dtype, device=dev)
-    if out.numel():
-        with on(dev):
-            nat.check(nat.load().ic_fp4_dequantize(
-                d.packed.data_ptr(), d.scales.data_ptr(), nat.ptr(d.row_scale), FORMATS[q.fmt], d.rows, d.columns,
-                _DT[dtype], out.data_ptr(), d.columns, nat.stream_ptr(dev)), "dequantize_fp4")
-    return back(out.reshape(*q.lead_shape(), d.columns), q.packed)
+    d = q if q.packed.is_cuda else q.to(dev)
+    rows, columns = d.rows, d.columns
+    out = torch.empty((rows, columns), dtype=dtype, device=dev)
+    if rows and columns:
+        call("ic_fp4_dequantize", dev, d.packed.data_ptr(), d.scales.data_ptr(), nat.ptr(d.row_scale), FORMATS[q.fmt], rows,
+             columns, _DT[dtype], out.data_ptr(), columns)
+    if q.lead is not None:
+        out = out.reshape(*q.lead, columns)
+    return back(out, q.packed)
 
 
 def check_bias(bias: torch.Tensor | None, n: int, dev: torch.device) -> torch.Tensor | None:
@@ -188,6 +194,8 @@ def check_bias(bias: torch.Tensor | None, n: int, dev: torch.device) -> torch.Te
         return None
     if bias.numel() != n or bias.dtype not in _DT:
         raise ValueError(f"bias must have {n} values in float32, float16 or bfloat16")
+    if bias.dim() == 1 and bias.device == dev and bias.is_contiguous():
+        return bias
     return bias.to(dev).reshape(-1).contiguous()
 
 
@@ -201,34 +209,31 @@ def matmul_fp4(a: FP4Tensor, b: FP4Tensor, bias: torch.Tensor | None = None,
     """
     a.check("matmul_fp4")
     b.check("matmul_fp4")
-    if a.fmt != b.fmt or a.columns != b.columns:
-        raise ValueError(f"matmul_fp4: operands differ: {a.fmt} with {a.columns} columns, {b.fmt} with {b.columns}")
+    pa, pb = a.packed, b.packed
+    m, half = pa.shape
+    n, half_b = pb.shape
+    if a.fmt != b.fmt or half != half_b:
+        raise ValueError(f"matmul_fp4: operands differ: {a.fmt} with {2 * half} columns, {b.fmt} with {2 * half_b}")
     if a.rot_size != b.rot_size:
         raise ValueError(f"matmul_fp4: operands are rotated by {a.rot_size} and {b.rot_size}")
-    if a.in_features is not None and b.in_features is not None and a.in_features != b.in_features:
+    if a.in_features != b.in_features and a.in_features is not None and b.in_features is not None:
         raise ValueError(f"matmul_fp4: operands have {a.in_features} and {b.in_features} input features")
-    if a.device != b.device:
+    device = pa.device
+    if device != pb.device:
         raise ValueError("matmul_fp4: operands are on different devices")
     if out_dtype not in _DT:
         raise ValueError(f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
-    dev = device_of(a.packed)
-    m, n = a.rows, b.rows
+    dev = device_of(pa)
     bias_d = check_bias(bias, n, dev)
-    on_cpu = not a.packed.is_cuda
-    if on_cpu:
-        da, db = a.to(dev), b.to(dev)
-    else:
-        da, db = a, b
-    y = torch.empty(m, n, dtype=out_dtype, device=dev)
+    da, db = (a, b) if pa.is_cuda else (a.to(dev), b.to(dev))
+    y = torch.empty((m, n), dtype=out_dtype, device=dev)
     if m and n:
-        if a.columns == 0:
+        if half == 0:
             y.zero_() if bias_d is None else y.copy_(bias_d.float().expand(m, n))
         else:
-            with on(dev):
-                nat.check(nat.load().ic_fp4_matmul(
-                    da.packed.data_ptr(), da.scales.data_ptr(), nat.ptr(da.row_scale), db.packed.data_ptr(),
-                    db.scales.data_ptr(), nat.ptr(db.row_scale), FORMATS[a.fmt], m, n, a.columns, nat.ptr(bias_d),
-                    0 if bias_d is None else _DT[bias_d.dtype], _DT[out_dtype], y.data_ptr(), n, nat.stream_ptr(dev)),
-                    "matmul_fp4")
-    y = y.reshape(*a.lead_shape(), n)
-    return y.to(a.device) if on_cpu else y
+            call("ic_fp4_matmul", dev, da.packed.data_ptr(), da.scales.data_ptr(), nat.ptr(da.row_scale),
+                 db.packed.data_ptr(), db.scales.data_ptr(), nat.ptr(db.row_scale), FORMATS[a.fmt], m, n, 2 * half,
+                 nat.ptr(bias_d), 0 if bias_d is None else _DT[bias_d.dtype], _DT[out_dtype], y.data_ptr(), n)
+    if a.lead is not None:
+        y = y.reshape(*a.lead, n)
+    return back(y, pa)

@@ -12,7 +12,7 @@ import dataclasses
 import torch
 
 from . import _native as nat
-from ._dev import back, device_of, on
+from ._dev import back, call, device_of
 from .fp4 import check_bias
 from .rotation import _DT
 
@@ -45,31 +45,38 @@ class Int8Rows:
     def device(self) -> torch.device:
         return self.codes.device
 
-    def lead_shape(self) -> tuple:
-        return (self.rows,) if self.lead is None else tuple(self.lead)
-
     def check(self, what: str) -> None:
-        if self.codes.dim() != 2 or self.codes.dtype != torch.int8:
+        c, s, t = self.codes, self.scales, self.sums
+        if c.dim() != 2 or c.dtype is not torch.int8:
             raise ValueError(f"{what}: codes must be int8 [rows, columns]")
-        if self.scales.dtype != torch.float32 or self.scales.numel() != self.rows:
+        rows, device = c.shape[0], c.device
+        if s.dtype is not torch.float32 or s.numel() != rows:
             raise ValueError(f"{what}: scales must be fp32 [rows, 1]")
-        if self.sums is not None and (self.sums.dtype != torch.int32 or self.sums.numel() != self.rows):
+        if t is not None and (t.dtype is not torch.int32 or t.numel() != rows):
             raise ValueError(f"{what}: sums must be int32 [rows]")
-        if self.scales.device != self.device or (self.sums is not None and self.sums.device != self.device):
+        if s.device != device or (t is not None and t.device != device):
             raise ValueError(f"{what}: codes, scales and sums must be on one device")
 
 
-def empty_int8(rows: int, columns: int, dev: torch.device, **kw) -> Int8Rows:
+def empty_int8(rows: int, columns: int, dev: torch.device, in_features: int | None = None, rot_size: int = 0,
+               lead: tuple | None = None) -> Int8Rows:
     """Int8Rows of uninitialised parts, rows at a pitch of a multiple of 16 bytes."""
-    buf = torch.empty(rows, (columns + 15) & ~15, dtype=torch.int8, device=dev)
-    return Int8Rows(buf[:, :columns], torch.empty(rows, 1, dtype=torch.float32, device=dev),
-                    torch.empty(rows, dtype=torch.int32, device=dev), **kw)
+    buf = torch.empty((rows, (columns + 15) & ~15), dtype=torch.int8, device=dev)
+    return Int8Rows(buf[:, :columns] if columns & 15 else buf, torch.empty((rows, 1), dtype=torch.float32, device=dev),
+                    torch.empty((rows,), dtype=torch.int32, device=dev), in_features, rot_size, lead)
+
+
+def flat(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """One value per row, as the kernels read them."""
+    if t.is_contiguous() and t.is_cuda:
+        return t
+    return t.to(dev).reshape(-1).contiguous()
 
 
 def pitched(codes: torch.Tensor, dev: torch.device) -> tuple[torch.Tensor, int]:
     """(codes on ``dev`` as the product reads them, row pitch): 16-byte aligned rows,
     copied when they are not."""
-    c = codes.to(dev)
+    c = codes if codes.is_cuda else codes.to(dev)
     rows, k = c.shape
     if (k == 1 or c.stride(1) == 1) and c.data_ptr() % 16 == 0:
         if rows == 1:
@@ -87,17 +94,19 @@ def dequantize_int8(q: Int8Rows, dtype: torch.dtype = torch.float32) -> torch.Te
     if dtype not in _DT:
         raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     dev = device_of(q.codes)
-    out = torch.empty(q.rows, q.columns, dtype=dtype, device=dev)
-    if out.numel():
-        with on(dev):
-            codes = q.codes.to(dev)
-            if codes.stride(1) != 1 or codes.stride(0) < q.columns:
-                codes = codes.contiguous()
-            scales = q.scales.to(dev).reshape(-1).contiguous()
-            nat.check(nat.load().ic_int8_dequantize(
-                codes.data_ptr(), max(codes.stride(0), q.columns), scales.data_ptr(), q.rows, q.columns, _DT[dtype],
-                out.data_ptr(), q.columns, nat.stream_ptr(dev)), "dequantize_int8")
-    return back(out.reshape(*q.lead_shape(), q.columns), q.codes)
+    rows, columns = q.codes.shape
+    out = torch.empty((rows, columns), dtype=dtype, device=dev)
+    if rows and columns:
+        codes = q.codes if q.codes.is_cuda else q.codes.to(dev)
+        pitch, step = codes.stride()
+        if step != 1 or pitch < columns:
+            codes = codes.contiguous()
+            pitch = columns
+        call("ic_int8_dequantize", dev, codes.data_ptr(), pitch, flat(q.scales, dev).data_ptr(), rows, columns, _DT[dtype],
+             out.data_ptr(), columns)
+    if q.lead is not None:
+        out = out.reshape(*q.lead, columns)
+    return back(out, q.codes)
 
 
 def matmul_int8(a: Int8Rows, w_codes: torch.Tensor, w_scales: torch.Tensor,
@@ -115,9 +124,9 @@ def matmul_int8(a: Int8Rows, w_codes: torch.Tensor, w_scales: torch.Tensor,
     a.check("matmul_int8")
     if w_codes.dim() != 2 or w_codes.dtype != torch.int8:
         raise ValueError("matmul_int8: w_codes must be int8 [out, columns]")
-    m, (n, k) = a.rows, w_codes.shape
-    if a.columns != k:
-        raise ValueError(f"matmul_int8: rows have {a.columns} columns, the weights {k}")
+    (m, ka), (n, k) = a.codes.shape, w_codes.shape
+    if ka != k:
+        raise ValueError(f"matmul_int8: rows have {ka} columns, the weights {k}")
     if k > (MAX_K if w_zero_points is None else MAX_K_ASYM):
         raise ValueError(f"matmul_int8: int32 sums hold {MAX_K} columns, {MAX_K_ASYM} with zero-points; got {k}")
     if w_scales.dtype != torch.float16 or w_scales.numel() != n:
@@ -126,31 +135,30 @@ def matmul_int8(a: Int8Rows, w_codes: torch.Tensor, w_scales: torch.Tensor,
         raise ValueError(f"matmul_int8: w_zero_points must be int8 with {n} values (one per row)")
     if out_dtype not in _DT:
         raise ValueError(f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
-    if any(t is not None and t.device != a.device for t in (w_codes, w_scales, w_zero_points)):
+    device = a.codes.device
+    if w_codes.device != device or w_scales.device != device or (w_zero_points is not None and w_zero_points.device != device):
         raise ValueError("matmul_int8: operands are on different devices")
     dev = device_of(a.codes)
     bias_d = check_bias(bias, n, dev)
-    y = torch.empty(m, n, dtype=out_dtype, device=dev)
+    y = torch.empty((m, n), dtype=out_dtype, device=dev)
     if m and n:
         if k == 0:
             y.zero_() if bias_d is None else y.copy_(bias_d.float().expand(m, n))
         else:
-            with on(dev):
-                st, lib = nat.stream_ptr(dev), nat.load()
-                x, ldx = pitched(a.codes, dev)
-                w, ldw = pitched(w_codes, dev)
-                s = a.scales.to(dev).reshape(-1).contiguous()
-                ws = w_scales.to(dev).reshape(-1).contiguous()
-                zp = sums = None
-                if w_zero_points is not None:
-                    zp = w_zero_points.to(dev).reshape(-1).contiguous()
-                    if a.sums is None:
-                        sums = torch.empty(m, dtype=torch.int32, device=dev)
-                        nat.check(lib.ic_int8_row_sums(x.data_ptr(), ldx, m, k, sums.data_ptr(), st), "matmul_int8")
-                    else:
-                        sums = a.sums.to(dev).reshape(-1).contiguous()
-                nat.check(lib.ic_int8_matmul(
-                    x.data_ptr(), ldx, s.data_ptr(), nat.ptr(sums), w.data_ptr(), ldw, ws.data_ptr(), nat.ptr(zp), m, n, k,
-                    nat.ptr(bias_d), 0 if bias_d is None else _DT[bias_d.dtype], _DT[out_dtype], y.data_ptr(), n, st),
-                    "matmul_int8")
-    return back(y.reshape(*a.lead_shape(), n), a.codes)
+            x, ldx = pitched(a.codes, dev)
+            w, ldw = pitched(w_codes, dev)
+            zp = sums = None
+            if w_zero_points is not None:
+                zp, sums = flat(w_zero_points, dev), a.sums
+                if sums is None:
+                    sums = torch.empty(m, dtype=torch.int32, device=dev)
+                    call("ic_int8_row_sums", dev, x.data_ptr(), ldx, m, k, sums.data_ptr())
+                else:
+                    sums = flat(sums, dev)
+            s, ws = flat(a.scales, dev), flat(w_scales, dev)
+            call("ic_int8_matmul", dev, x.data_ptr(), ldx, s.data_ptr(), nat.ptr(sums), w.data_ptr(), ldw, ws.data_ptr(),
+                 nat.ptr(zp), m, n, k, nat.ptr(bias_d), 0 if bias_d is None else _DT[bias_d.dtype], _DT[out_dtype],
+                 y.data_ptr(), n)
+    if a.lead is not None:
+        y = y.reshape(*a.lead, n)
+    return back(y, a.codes)

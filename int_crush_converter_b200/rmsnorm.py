@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as nat
-from ._dev import back, device_of, on
+from ._dev import back, call, device_of
 from .fp4 import FORMATS, FP4Tensor, as_rows, empty_fp4, padded_columns, pitch
 from .int8 import Int8Rows, empty_int8
 from .rotation import _DT
@@ -43,27 +43,25 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
     dev = device_of(x)
-    lead = tuple(x.shape[:-1])
-    with on(dev):
-        x2 = as_rows(x, dev)
-        r2 = None if residual is None else as_rows(residual, dev)
-        w = weight.to(dev).reshape(-1).contiguous()
-        rows, kp = x2.shape[0], padded_columns(k, fmt, rot_size)
-        h = None if residual is None else torch.empty(rows, k, dtype=x.dtype, device=dev)
-        if fmt == "int8":
-            q = empty_int8(rows, kp, dev, in_features=k, rot_size=rot_size, lead=lead)
-            codes, ldq, scales, row, sums = q.codes, (kp + 15) & ~15, None, q.scales, q.sums
-        else:
-            q = empty_fp4(rows, kp, fmt, dev, in_features=k, rot_size=rot_size, lead=lead)
-            codes, ldq, scales, row, sums = q.packed, kp // 2, q.scales, q.row_scale, None
-        if rows:
-            nat.check(nat.load().ic_rmsnorm_quantize(
-                x2.data_ptr(), nat.ptr(r2), _DT[x.dtype], rows, k, pitch(x2), 0 if r2 is None else pitch(r2), w.data_ptr(),
-                _DT[w.dtype], float(eps), _FORMATS[fmt], rot_size, kp, nat.ptr(h), k, codes.data_ptr(), ldq,
-                nat.ptr(scales), nat.ptr(row), nat.ptr(sums), nat.stream_ptr(dev)), "rmsnorm_quantize")
+    lead = x.shape[:-1]
+    x2 = as_rows(x, dev)
+    r2 = None if residual is None else as_rows(residual, dev)
+    w = weight if weight.is_cuda and weight.is_contiguous() else weight.to(dev).reshape(-1).contiguous()
+    rows, kp = x2.shape[0], padded_columns(k, fmt, rot_size)
+    h = None if residual is None else torch.empty((rows, k), dtype=x.dtype, device=dev)
+    if fmt == "int8":
+        q = empty_int8(rows, kp, dev, k, rot_size, lead)
+        codes, ldq, scales, row, sums = q.codes, (kp + 15) & ~15, None, q.scales, q.sums
+    else:
+        q = empty_fp4(rows, kp, fmt, dev, k, rot_size, lead)
+        codes, ldq, scales, row, sums = q.packed, kp // 2, q.scales, q.row_scale, None
+    if rows:
+        call("ic_rmsnorm_quantize", dev, x2.data_ptr(), nat.ptr(r2), _DT[x.dtype], rows, k, pitch(x2),
+             0 if r2 is None else pitch(r2), w.data_ptr(), _DT[w.dtype], float(eps), _FORMATS[fmt], rot_size, kp, nat.ptr(h), k,
+             codes.data_ptr(), ldq, nat.ptr(scales), nat.ptr(row), nat.ptr(sums))
     if not x.is_cuda:
         if fmt == "int8":
             q.codes, q.scales, q.sums = q.codes.to(x.device), q.scales.to(x.device), q.sums.to(x.device)
         else:
             q = q.to(x.device)
-    return q, None if h is None else back(h.reshape(x.shape), x)
+    return q, None if h is None else back(h.view(x.shape), x)
