@@ -147,6 +147,26 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])     \
       : "r"(taddr))
 
+#define IC_TMEM_LD32(taddr, r)                                                                   \
+  asm volatile(                                                                                  \
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"   \
+      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"         \
+      : "=r"((r)[0]), "=r"((r)[1]), "=r"((r)[2]), "=r"((r)[3]), "=r"((r)[4]), "=r"((r)[5]),      \
+        "=r"((r)[6]), "=r"((r)[7]), "=r"((r)[8]), "=r"((r)[9]), "=r"((r)[10]), "=r"((r)[11]),    \
+        "=r"((r)[12]), "=r"((r)[13]), "=r"((r)[14]), "=r"((r)[15]), "=r"((r)[16]), "=r"((r)[17]), \
+        "=r"((r)[18]), "=r"((r)[19]), "=r"((r)[20]), "=r"((r)[21]), "=r"((r)[22]), "=r"((r)[23]), \
+        "=r"((r)[24]), "=r"((r)[25]), "=r"((r)[26]), "=r"((r)[27]), "=r"((r)[28]), "=r"((r)[29]), \
+        "=r"((r)[30]), "=r"((r)[31])                                                             \
+      : "r"(taddr))
+
+// What the epilogue applies to a 128 x BN tile: one side of it belongs to the
+// activations (factor, sum of codes), the other to the weights (factor, bias,
+// zero-point).
+struct TileFactors {
+  float rowf[128], rowb[128], colf[256], colb[256];
+  int rowi[128], coli[256];
+};
+
 template <int KIND, int BN>
 struct Cfg {
   static constexpr bool FP4 = KIND != IC_INT8;
@@ -159,13 +179,14 @@ struct Cfg {
   static constexpr int STAGE_BYTES = P_BYTES + Q_BYTES + PS_BYTES + QS_BYTES;
   // narrow tiles leave room for two CTAs on an SM; wide ones take the SM
   static constexpr int CTAS = BN <= 64 ? 2 : 1;
-  static constexpr int STAGES = (CTAS == 2 ? 98304 : 212992) / STAGE_BYTES;
+  static constexpr int STAGES = (CTAS == 2 ? 98304 : 222000) / STAGE_BYTES;
   static constexpr int SF_COLS = SF_TILES * 4 * (1 + Q_ATOMS);  // TMEM columns of one stage's scales
   static constexpr int ACC_COLS = BN < 32 ? 32 : BN;
   static constexpr int TMEM_NEED = ACC_COLS + STAGES * SF_COLS;
   static constexpr int TMEM_COLS = TMEM_NEED <= 32 ? 32 : TMEM_NEED <= 64 ? 64 : TMEM_NEED <= 128 ? 128 : TMEM_NEED <= 256 ? 256 : 512;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 /*align*/ + 512 /*barriers*/;
+  static constexpr int SMEM = STAGES * STAGE_BYTES + (int)sizeof(TileFactors) + 1024 /*align*/ + 256 /*barriers*/;
   static_assert(TMEM_NEED <= 512 / CTAS, "tensor memory");
+  static_assert(SMEM <= 232448 / CTAS, "shared memory");
   static_assert(BM * BN * 4 <= STAGES * STAGE_BYTES, "a partial tile fits in the stages");
   static constexpr uint32_t IDESC =
       KIND == IC_INT8 ? (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24)
@@ -198,28 +219,184 @@ __device__ __forceinline__ void load_strided(const void* p, int type, int first,
       if (first + 32 * i < limit) v[i] = __bfloat162float(static_cast<const __nv_bfloat16*>(p)[first + 32 * i]);
   }
 }
-__device__ __forceinline__ void store_any(void* p, int type, long long i, float v) {
-  if (type == IC_F32) static_cast<float*>(p)[i] = v;
-  else if (type == IC_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+// One sum to its output: fp32 scaling in a fixed order (zero-point, the
+// activations' factor, the weights' factor, bias), rounded to the output type
+// once, by the caller.
+template <int KIND>
+__device__ __forceinline__ float finish(uint32_t acc, int zs, float tokf, float wf, float bias, bool has_bias) {
+  float v = KIND == IC_INT8 ? (float)((int)acc - zs) : __uint_as_float(acc);
+  if (KIND != IC_MXFP4) v = __fmul_rn(__fmul_rn(v, tokf), wf);
+  return has_bias ? __fadd_rn(v, bias) : v;
+}
+template <typename T>
+__device__ __forceinline__ T to_out(float v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
+  else return __float2bfloat16_rn(v);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* to, const T (&e)[V]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(e);
+  if constexpr (V * sizeof(T) == 32)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  else
+    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(e);
 }
 
-// y[token, n] of one sum: fp32 scaling in a fixed order, one rounding to the output type at the end
-template <int KIND>
-__device__ __forceinline__ float finish(const LowpArgs& a, uint32_t acc, int token, int n, const void* tok_row, int tok_half,
-                                        const void* w_row, int w_half) {
-  float v;
-  if (KIND == IC_INT8) {
-    int s = (int)acc;
-    if (a.zp) s -= (int)a.zp[n] * a.sums[token];
-    v = (float)s;
-  } else {
-    v = __uint_as_float(acc);
+// factors of a tile's rows and columns, by 128 threads
+template <int BN>
+__device__ __forceinline__ void load_factors(const LowpArgs& a, TileFactors& f, int p0, int q0, int t) {
+  const int row = p0 + t;
+  const bool in = row < a.pm;
+  f.rowf[t] = in && a.p_row ? load_any(a.p_row, a.p_half ? IC_F16 : IC_F32, row) : 0.f;
+  f.rowb[t] = in && a.swap && a.bias ? load_any(a.bias, a.bias_type, row) : 0.f;
+  f.rowi[t] = in && a.zp ? (a.swap ? (int)a.zp[row] : a.sums[row]) : 0;
+#pragma unroll
+  for (int i = 0; i < (BN + 127) / 128; ++i) {
+    const int c = i * 128 + t, col = q0 + c;
+    if (c >= BN) break;
+    const bool on = col < a.qn;
+    f.colf[c] = on && a.q_row ? load_any(a.q_row, a.q_half ? IC_F16 : IC_F32, col) : 0.f;
+    f.colb[c] = on && !a.swap && a.bias ? load_any(a.bias, a.bias_type, col) : 0.f;
+    f.coli[c] = on && a.zp ? (a.swap ? a.sums[col] : (int)a.zp[col]) : 0;
   }
-  if (tok_row) v = __fmul_rn(v, load_any(tok_row, tok_half ? IC_F16 : IC_F32, token));
-  if (w_row) v = __fmul_rn(v, load_any(w_row, w_half ? IC_F16 : IC_F32, n));
-  if (a.bias) v = __fadd_rn(v, load_any(a.bias, a.bias_type, n));
-  return v;
+}
+
+// This CTA's share of a split tile's columns: the S partial sums in rank order, then to y
+template <int KIND, int BN, int S, typename T>
+__device__ __forceinline__ void add_parts(const LowpArgs& a, const TileFactors& f, T* y, const uint32_t* part, int p0, int q0,
+                                          int rank) {
+  constexpr int SHARE = BN / S, V = SHARE < 16 / (int)sizeof(T) ? SHARE : 16 / (int)sizeof(T);  // columns: in all, at a time
+  const int lr = threadIdx.x & 127, row = p0 + lr, c0 = rank * SHARE, left = min(SHARE, a.qn - q0 - c0);
+  uint32_t peer[S];
+#pragma unroll
+  for (int r = 0; r < S; ++r) peer[r] = map_to_rank(smem_u32(part + c0 * BM + lr), r);
+  const float rowf = f.rowf[lr], rowb = f.rowb[lr];
+  const int rowi = f.rowi[lr];
+  const bool has_bias = a.bias != nullptr;
+  const bool vec = !a.swap && V * sizeof(T) == 16 && ((reinterpret_cast<uintptr_t>(y) | (uintptr_t)(a.ldy * (long long)sizeof(T))) & 15) == 0;
+  for (int g = (threadIdx.x >> 7) * V; g < left; g += 2 * V) {
+    uint32_t v[V][S];  // all loads in flight together
+#pragma unroll
+    for (int u = 0; u < V; ++u)
+#pragma unroll
+      for (int r = 0; r < S; ++r) v[u][r] = ld_cluster(peer[r] + (uint32_t)((g + u) * BM) * 4u);
+    alignas(16) T e[V];
+#pragma unroll
+    for (int u = 0; u < V; ++u) {
+      const int c = c0 + g + u;
+      uint32_t s = v[u][0];
+#pragma unroll
+      for (int r = 1; r < S; ++r) {
+        if (KIND == IC_INT8) s += v[u][r];
+        else s = __float_as_uint(__fadd_rn(__uint_as_float(s), __uint_as_float(v[u][r])));
+      }
+      const float cf = f.colf[c];
+      e[u] = to_out<T>(finish<KIND>(s, rowi * f.coli[c], a.swap ? cf : rowf, a.swap ? rowf : cf, a.swap ? rowb : f.colb[c], has_bias));
+    }
+    if (row >= a.pm) continue;
+    const int col = q0 + c0 + g;
+    if (a.swap) {
+#pragma unroll
+      for (int u = 0; u < V; ++u)
+        if (g + u < left) y[(long long)(col + u) * a.ldy + row] = e[u];
+    } else if (vec && g + V <= left && col % V == 0) {
+      if constexpr (V * sizeof(T) == 16) store_vec<T, V>(y + (long long)row * a.ldy + col, e);
+    } else {
+#pragma unroll
+      for (int u = 0; u < V; ++u)
+        if (g + u < left) y[(long long)row * a.ldy + col + u] = e[u];
+    }
+  }
+}
+
+// Sums to y.  The accumulator's lanes are rows of P, its columns rows of Q.
+//  - one CTA per tile, activations in P: each lane stores pieces of its own row
+//    of y (whole sectors where the rows are aligned; otherwise through shared
+//    memory, neighbouring lanes storing neighbouring elements);
+//  - weights in P: lanes are neighbouring columns of y, stored as they are;
+//  - split K: partial tiles go to shared memory as [column][128 rows], each CTA
+//    of the cluster adds its share of the columns over the CTAs in rank order.
+template <int KIND, int BN, typename T>
+__device__ __forceinline__ void epilogue(const LowpArgs& a, const TileFactors& f, unsigned char* smem, uint32_t tmem,
+                                         uint32_t acc_bar, int p0, int q0, int rank) {
+  constexpr int W = BN < 32 ? 16 : 32;  // columns at a time
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3;
+  T* y = static_cast<T*>(a.y);
+  const bool has_bias = a.bias != nullptr;
+  uint32_t* part = reinterpret_cast<uint32_t*>(smem);
+  if (warp >= 4) {
+    asm volatile("bar.sync 1, 128;" ::: "memory");  // the factors are written
+    bool ok = warp_wait(acc_bar, 0, a.flags);
+    if (!ok) warp_wait(acc_bar, 0, a.flags);  // products in flight end before their tensor memory is freed
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    const int lr = q * 32 + lane, row = p0 + lr;
+    const float rowf = f.rowf[lr], rowb = f.rowb[lr];
+    const int rowi = f.rowi[lr];
+    constexpr int V = 32 / sizeof(T);
+    const bool vec = !a.swap && ((reinterpret_cast<uintptr_t>(y) | (uintptr_t)(a.ldy * (long long)sizeof(T))) & 31) == 0;
+    const int cols = min(BN, a.qn - q0);
+    for (int c = 0; c < cols; c += W) {
+      uint32_t r[W];
+      const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c;
+      if constexpr (W == 16) IC_TMEM_LD16(at, r);
+      else IC_TMEM_LD32(at, r);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      if (a.splits > 1) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) part[(c + j) * BM + lr] = r[j];
+        continue;
+      }
+      if (!ok) continue;
+      float v[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const float cf = f.colf[c + j];
+        v[j] = finish<KIND>(r[j], rowi * f.coli[c + j], a.swap ? cf : rowf, a.swap ? rowf : cf, a.swap ? rowb : f.colb[c + j], has_bias);
+      }
+      if (a.swap) {
+        if (row < a.pm) {
+          T* to = y + (long long)(q0 + c) * a.ldy + row;
+#pragma unroll
+          for (int j = 0; j < W; ++j)
+            if (c + j < cols) to[j * a.ldy] = to_out<T>(v[j]);
+        }
+      } else if (vec) {
+        T* to = y + (long long)row * a.ldy + q0 + c;
+        const int left = row < a.pm ? cols - c : 0;
+#pragma unroll
+        for (int j = 0; j < W; j += V) {
+          alignas(32) T e[V];
+#pragma unroll
+          for (int u = 0; u < V; ++u) e[u] = to_out<T>(v[j + u]);
+          if (j + V <= left) store_vec<T, V>(to + j, e);
+          else
+#pragma unroll
+            for (int u = 0; u < V; ++u)
+              if (j + u < left) to[j + u] = e[u];
+        }
+      } else {
+        // the stages are idle by now; 33 elements to a row keep the banks apart
+        T* mine = reinterpret_cast<T*>(smem) + q * (32 * 34);
+#pragma unroll
+        for (int j = 0; j < W; ++j) mine[lane * 34 + j] = to_out<T>(v[j]);
+        __syncwarp();
+        const int rows = min(32, a.pm - p0 - q * 32), wide = min(W, cols - c);
+        if (lane < wide)
+          for (int i = 0; i < rows; ++i) y[(long long)(p0 + q * 32 + i) * a.ldy + q0 + c + lane] = mine[i * 34 + lane];
+        __syncwarp();
+      }
+    }
+  }
+  if (a.splits > 1) {
+    cluster_sync();
+    if (a.splits == 2) add_parts<KIND, BN, 2>(a, f, y, part, p0, q0, rank);
+    else if (a.splits == 4) add_parts<KIND, BN, 4>(a, f, y, part, p0, q0, rank);
+    else add_parts<KIND, BN, 8>(a, f, y, part, p0, q0, rank);
+    cluster_sync();  // no CTA leaves while a peer reads its partial tile
+  }
 }
 
 constexpr int GROUP = 16;  // row tiles per group of the tile order: a wave of CTAs reads a compact patch of P and Q
@@ -231,7 +408,8 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
   constexpr int STAGES = C::STAGES;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE_BYTES);
+  TileFactors& f = *reinterpret_cast<TileFactors*>(smem + STAGES * C::STAGE_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE_BYTES + sizeof(TileFactors));
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 1);
   auto full_bar = [&](int s) { return smem_u32(bars + s); };
   auto empty_bar = [&](int s) { return smem_u32(bars + STAGES + s); };
@@ -274,7 +452,7 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
       const uint32_t base = smem_u32(smem + s * C::STAGE_BYTES);
       uint32_t bytes = C::P_BYTES + C::Q_BYTES, sf = 0;
       const int rt = q0 >> 7;
-      const bool two = C::Q_ATOMS == 2 && q0 + BM < a.qn;
+      const bool two = C::Q_ATOMS == 2 && (rt + 1) * BM < a.qn;
       if (C::FP4) {
         sf = (uint32_t)min(C::SF_TILES, a.ktiles - kt * C::SF_TILES) * 512u;  // at least one tile: kt is within K
         bytes += sf * (two ? 3u : 2u);
@@ -338,54 +516,10 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
   __syncwarp();
 
   // ---------------- epilogue ----------------
-  const void *tok_row = a.swap ? a.q_row : a.p_row, *w_row = a.swap ? a.p_row : a.q_row;
-  const int tok_half = a.swap ? a.q_half : a.p_half, w_half = a.swap ? a.p_half : a.q_half;
-  const int q = warp & 3;
-  uint32_t* part = reinterpret_cast<uint32_t*>(smem);  // [column][128 rows]
-  if (warp >= 4) {
-    bool ok = mbar_wait(acc_bar, 0, a.flags);
-    if (!ok) mbar_wait(acc_bar, 0, a.flags);  // products in flight end before their tensor memory is freed
-    asm volatile("tcgen05.fence::after_thread_sync;");
-    const int row = p0 + q * 32 + lane;
-    for (int c = 0; c < BN; c += 16) {
-      uint32_t r[16];
-      IC_TMEM_LD16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      if (a.splits > 1) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) part[(c + j) * BM + q * 32 + lane] = r[j];
-      } else if (ok && row < a.pm) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int col = q0 + c + j;
-          if (col < a.qn) {
-            const int token = a.swap ? col : row, w = a.swap ? row : col;
-            store_any(a.y, a.out_type, (long long)token * a.ldy + w, finish<KIND>(a, r[j], token, w, tok_row, tok_half, w_row, w_half));
-          }
-        }
-      }
-    }
-  }
-  if (a.splits > 1) {
-    cluster_sync();
-    const int c0 = rank * BN / a.splits, c1 = (rank + 1) * BN / a.splits;
-    for (int i = threadIdx.x; i < (c1 - c0) * BM; i += blockDim.x) {
-      const int c = c0 + i / BM, lrow = i % BM, row = p0 + lrow, col = q0 + c;
-      if (row >= a.pm || col >= a.qn) continue;
-      const uint32_t at = smem_u32(part + c * BM + lrow);
-      uint32_t s = 0;
-      float f = 0.f;
-      for (int r = 0; r < a.splits; ++r) {
-        const uint32_t v = ld_cluster(map_to_rank(at, r));
-        if (KIND == IC_INT8) s += v;
-        else f = __fadd_rn(f, __uint_as_float(v));
-      }
-      if (KIND != IC_INT8) s = __float_as_uint(f);
-      const int token = a.swap ? col : row, w = a.swap ? row : col;
-      store_any(a.y, a.out_type, (long long)token * a.ldy + w, finish<KIND>(a, s, token, w, tok_row, tok_half, w_row, w_half));
-    }
-    cluster_sync();  // no CTA leaves while a peer reads its partial tile
-  }
+  if (warp >= 4) load_factors<BN>(a, f, p0, q0, threadIdx.x - 128);
+  if (a.out_type == IC_BF16) epilogue<KIND, BN, __nv_bfloat16>(a, f, smem, tmem, acc_bar, p0, q0, rank);
+  else if (a.out_type == IC_F16) epilogue<KIND, BN, __half>(a, f, smem, tmem, acc_bar, p0, q0, rank);
+  else epilogue<KIND, BN, float>(a, f, smem, tmem, acc_bar, p0, q0, rank);
   asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
   if (warp == 2) {
@@ -495,18 +629,6 @@ __device__ __forceinline__ void remote_arrive(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-#define IC_TMEM_LD32(taddr, r)                                                                   \
-  asm volatile(                                                                                  \
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"   \
-      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"         \
-      : "=r"((r)[0]), "=r"((r)[1]), "=r"((r)[2]), "=r"((r)[3]), "=r"((r)[4]), "=r"((r)[5]),      \
-        "=r"((r)[6]), "=r"((r)[7]), "=r"((r)[8]), "=r"((r)[9]), "=r"((r)[10]), "=r"((r)[11]),    \
-        "=r"((r)[12]), "=r"((r)[13]), "=r"((r)[14]), "=r"((r)[15]), "=r"((r)[16]), "=r"((r)[17]), \
-        "=r"((r)[18]), "=r"((r)[19]), "=r"((r)[20]), "=r"((r)[21]), "=r"((r)[22]), "=r"((r)[23]), \
-        "=r"((r)[24]), "=r"((r)[25]), "=r"((r)[26]), "=r"((r)[27]), "=r"((r)[28]), "=r"((r)[29]), \
-        "=r"((r)[30]), "=r"((r)[31])                                                             \
-      : "r"(taddr))
-
 // One lane's row of four sums from column c of the tile, scaled
 template <int KIND>
 __device__ __forceinline__ void finish4(const LowpArgs& a, const uint32_t* acc, const Factors& f, int c, float rowf, int sum,
@@ -517,18 +639,8 @@ __device__ __forceinline__ void finish4(const LowpArgs& a, const uint32_t* acc, 
   int z[4];
   if (KIND == IC_INT8 && a.zp) *reinterpret_cast<int4*>(z) = *reinterpret_cast<const int4*>(f.zp + c);
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    if (KIND == IC_INT8) v[u] = (float)((int)acc[u] - (a.zp ? z[u] * sum : 0));
-    else v[u] = __uint_as_float(acc[u]);
-    if (KIND != IC_MXFP4) v[u] = __fmul_rn(__fmul_rn(v[u], rowf), s[u]);
-    if (a.bias) v[u] = __fadd_rn(v[u], b[u]);
-  }
-}
-template <typename T>
-__device__ __forceinline__ T to_out(float v) {
-  if constexpr (sizeof(T) == 4) return v;
-  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
-  else return __float2bfloat16_rn(v);
+  for (int u = 0; u < 4; ++u)
+    v[u] = finish<KIND>(acc[u], KIND == IC_INT8 && a.zp ? z[u] * sum : 0, rowf, s[u], a.bias ? b[u] : 0.f, a.bias != nullptr);
 }
 
 // One warp's 32 rows x 128 columns of sums, from column c0 of the tile, to y.
@@ -557,10 +669,7 @@ __device__ __forceinline__ void store_block(const LowpArgs& a, const uint32_t (&
         for (int w = 0; w < 4; ++w) e[u + w] = to_out<T>(v[w]);
       }
       if (c + V <= left) {
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(e);
-        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + c), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                     "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                     : "memory");
+        store_vec<T, V>(to + c, e);
       } else {
 #pragma unroll
         for (int u = 0; u < V; ++u)
@@ -853,7 +962,7 @@ struct Operand {
 };
 
 template <int KIND, int BN>
-int launch(const Operand& p, const Operand& q, LowpArgs a, cudaStream_t st) {
+int launch(const Operand& p, const Operand& q, LowpArgs a, int splits, cudaStream_t st) {
   using C = Cfg<KIND, BN>;
   static std::atomic<unsigned long long> done{0};
   IC_TRY(once_per_device(done, [] {
@@ -866,20 +975,17 @@ int launch(const Operand& p, const Operand& q, LowpArgs a, cudaStream_t st) {
   a.pm = (int)p.rows, a.qn = (int)q.rows;
   a.p_scales = p.scales, a.q_scales = q.scales;
   a.p_row = p.row, a.q_row = q.row, a.p_half = p.half, a.q_half = q.half;
+  a.splits = splits;
   const int64_t tiles = cdiv(p.rows, BM) * cdiv(q.rows, BN);
-  const int64_t stages = cdiv(a.kbytes, ROW_BYTES);
-  // split K while the split grid still fits the 148 SMs at once
-  a.splits = 1;
-  while (a.splits < MAX_SPLIT && tiles * a.splits * 2 <= 148 * C::CTAS && stages >= a.splits * 2) a.splits *= 2;
-  if (tiles * a.splits > INT32_MAX) return fail(IC_ERR_UNSUPPORTED, "matmul: too many tiles");
+  if (tiles * splits > INT32_MAX) return fail(IC_ERR_UNSUPPORTED, "matmul: too many tiles");
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(tiles * a.splits), 1, 1);
+  cfg.gridDim = dim3((unsigned)(tiles * splits), 1, 1);
   cfg.blockDim = dim3(256, 1, 1);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)a.splits;
+  attr[0].val.clusterDim.x = (unsigned)splits;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
@@ -953,17 +1059,62 @@ int launch_pair(const Operand& p, const Operand& q, LowpArgs a, cudaStream_t st)
   return IC_OK;
 }
 
-// x [m, k] times w [n, k]^T.  Up to 128 activation rows the weights take the
-// 128-row side and the activations a tile as narrow as they are.
+// How a product is cut: tile width, orientation and K split
+struct Plan {
+  int bn;      // 256-row pairs when 0
+  bool swap;   // the weights take the 128-row side
+  int splits;
+  double clocks;
+};
+
+// Estimated SM clocks of a one-CTA plan.  A stage takes the longer of its
+// products (BN/2 clocks for each of four) and its loads (63 bytes a clock and
+// SM, measured with all SMs loading from L2); a CTA's start, first loads and
+// epilogue take about 4000 clocks, a split's exchange about 1000 more.
+template <int KIND, int BN>
+void consider(Plan& best, int64_t pm, int64_t qn, int64_t stages, bool swap) {
+  using C = Cfg<KIND, BN>;
+  const int64_t tiles = cdiv(pm, BM) * cdiv(qn, BN);
+  for (int s = 1; s <= MAX_SPLIT && s <= stages; s *= 2) {
+    const int64_t ctas = tiles * s, waves = cdiv(ctas, 148 * C::CTAS);
+    const int per_sm = (int)std::min<int64_t>(C::CTAS, cdiv(ctas, 148));
+    const double stage = std::max(2.0 * BN, C::STAGE_BYTES / 63.0) * per_sm;
+    const double clocks = waves * ((double)cdiv(stages, s) * stage + 4000 + 8.0 * BN + (s > 1 ? 1000 + 2.0 * BN : 0));
+    if (clocks < best.clocks) best = Plan{BN, swap, s, clocks};
+  }
+}
+
+template <int KIND>
+Plan plan(int64_t m, int64_t n, int64_t stages) {
+  // pairs: 620 clocks a stage and 3000 between tiles (measured), a longer start
+  Plan best{0, false, 1, cdiv(cdiv(m, 256) * cdiv(n, 256), 74) * (stages * 620.0 + 3000) + 5000};
+  for (int swap = 0; swap < 2; ++swap) {
+    const int64_t pm = swap ? n : m, qn = swap ? m : n;
+    if (qn <= 16) consider<KIND, 16>(best, pm, qn, stages, swap);
+    if (qn <= 32) consider<KIND, 32>(best, pm, qn, stages, swap);
+    consider<KIND, 64>(best, pm, qn, stages, swap);
+    consider<KIND, 128>(best, pm, qn, stages, swap);
+    consider<KIND, 192>(best, pm, qn, stages, swap);
+    consider<KIND, 256>(best, pm, qn, stages, swap);
+  }
+  return best;
+}
+
+// x [m, k] times w [n, k]^T
 template <int KIND>
 int matmul(const Operand& x, const Operand& w, LowpArgs a, cudaStream_t st) {
-  a.swap = x.rows <= 128;
-  if (!a.swap && cdiv(x.rows, 256) * cdiv(w.rows, 256) >= 74) return launch_pair<KIND>(x, w, a, st);
-  if (!a.swap) return launch<KIND, 128>(x, w, a, st);
-  if (x.rows <= 16) return launch<KIND, 16>(w, x, a, st);
-  if (x.rows <= 32) return launch<KIND, 32>(w, x, a, st);
-  if (x.rows <= 64) return launch<KIND, 64>(w, x, a, st);
-  return launch<KIND, 128>(w, x, a, st);
+  const Plan b = plan<KIND>(x.rows, w.rows, cdiv(a.kbytes, ROW_BYTES));
+  a.swap = b.swap;
+  const Operand &p = b.swap ? w : x, &q = b.swap ? x : w;
+  switch (b.bn) {
+    case 16: return launch<KIND, 16>(p, q, a, b.splits, st);
+    case 32: return launch<KIND, 32>(p, q, a, b.splits, st);
+    case 64: return launch<KIND, 64>(p, q, a, b.splits, st);
+    case 128: return launch<KIND, 128>(p, q, a, b.splits, st);
+    case 192: return launch<KIND, 192>(p, q, a, b.splits, st);
+    case 256: return launch<KIND, 256>(p, q, a, b.splits, st);
+    default: return launch_pair<KIND>(x, w, a, st);
+  }
 }
 
 int check_product(const char* what, int64_t m, int64_t n, int64_t k, const void* bias, int bias_dtype, int out_dtype,

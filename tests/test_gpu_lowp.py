@@ -314,7 +314,9 @@ PRODUCTS = [
     (129, 128, 320, torch.bfloat16, False), (300, 520, 2080, torch.float32, True), (257, 1024, 4096, torch.bfloat16, True),
     (1, 4096, 16384, torch.bfloat16, False), (1000, 77, 640, torch.float16, False), (5, 3000, 32, torch.float32, False),
     (2304, 2200, 800, torch.bfloat16, True), (2400, 2177, 1433, torch.float16, True), (4700, 1300, 320, torch.float32, False),
-    (2305, 2304, 4096, torch.float32, True),
+    (2305, 2304, 4096, torch.float32, True), (300, 4096, 4096, torch.bfloat16, True), (700, 600, 2048, torch.float16, True),
+    (180, 5000, 1024, torch.float32, False), (1024, 1024, 512, torch.bfloat16, True), (90, 12288, 256, torch.float16, True),
+    (520, 333, 8192, torch.bfloat16, True),
 ]
 
 
