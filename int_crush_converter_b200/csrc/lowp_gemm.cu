@@ -1070,32 +1070,36 @@ struct Plan {
 // Estimated SM clocks of a one-CTA plan.  A stage takes the longer of its
 // products (BN/2 clocks for each of four) and its loads (63 bytes a clock and
 // SM, measured with all SMs loading from L2); a CTA's start, first loads and
-// epilogue take about 4000 clocks, a split's exchange about 1000 more.
+// epilogue take about 4000 clocks and 8 a column, a split's exchange 2500 and 12
+// a column, element stores into rows that are not 32-byte aligned 20 a column.
+// (Over 24 products from 1 x 4096 x 4096 to 2048 x 12288 x 4096, every plan
+// timed: the choice is within 10% of the fastest.)
 template <int KIND, int BN>
-void consider(Plan& best, int64_t pm, int64_t qn, int64_t stages, bool swap) {
+void consider(Plan& best, int64_t pm, int64_t qn, int64_t stages, bool swap, bool aligned) {
   using C = Cfg<KIND, BN>;
   const int64_t tiles = cdiv(pm, BM) * cdiv(qn, BN);
   for (int s = 1; s <= MAX_SPLIT && s <= stages; s *= 2) {
     const int64_t ctas = tiles * s, waves = cdiv(ctas, 148 * C::CTAS);
     const int per_sm = (int)std::min<int64_t>(C::CTAS, cdiv(ctas, 148));
     const double stage = std::max(2.0 * BN, C::STAGE_BYTES / 63.0) * per_sm;
-    const double clocks = waves * ((double)cdiv(stages, s) * stage + 4000 + 8.0 * BN + (s > 1 ? 1000 + 2.0 * BN : 0));
+    const double ends = 4000 + 8.0 * BN + (s > 1 ? 2500 + 12.0 * BN : 0) + (swap || aligned ? 0 : 20.0 * BN / s);
+    const double clocks = waves * ((double)cdiv(stages, s) * stage + ends);
     if (clocks < best.clocks) best = Plan{BN, swap, s, clocks};
   }
 }
 
 template <int KIND>
-Plan plan(int64_t m, int64_t n, int64_t stages) {
-  // pairs: 620 clocks a stage and 3000 between tiles (measured), a longer start
-  Plan best{0, false, 1, cdiv(cdiv(m, 256) * cdiv(n, 256), 74) * (stages * 620.0 + 3000) + 5000};
+Plan plan(int64_t m, int64_t n, int64_t stages, bool aligned) {
+  // pairs: 620 clocks a stage and 3000 between tiles, or an epilogue of element stores; a longer start (measured)
+  Plan best{0, false, 1, cdiv(cdiv(m, 256) * cdiv(n, 256), 74) * std::max(stages * 620.0 + 3000, aligned ? 0.0 : 25000.0) + 5000};
   for (int swap = 0; swap < 2; ++swap) {
     const int64_t pm = swap ? n : m, qn = swap ? m : n;
-    if (qn <= 16) consider<KIND, 16>(best, pm, qn, stages, swap);
-    if (qn <= 32) consider<KIND, 32>(best, pm, qn, stages, swap);
-    consider<KIND, 64>(best, pm, qn, stages, swap);
-    consider<KIND, 128>(best, pm, qn, stages, swap);
-    consider<KIND, 192>(best, pm, qn, stages, swap);
-    consider<KIND, 256>(best, pm, qn, stages, swap);
+    if (qn <= 16) consider<KIND, 16>(best, pm, qn, stages, swap, aligned);
+    if (qn <= 32) consider<KIND, 32>(best, pm, qn, stages, swap, aligned);
+    consider<KIND, 64>(best, pm, qn, stages, swap, aligned);
+    consider<KIND, 128>(best, pm, qn, stages, swap, aligned);
+    consider<KIND, 192>(best, pm, qn, stages, swap, aligned);
+    consider<KIND, 256>(best, pm, qn, stages, swap, aligned);
   }
   return best;
 }
@@ -1103,7 +1107,9 @@ Plan plan(int64_t m, int64_t n, int64_t stages) {
 // x [m, k] times w [n, k]^T
 template <int KIND>
 int matmul(const Operand& x, const Operand& w, LowpArgs a, cudaStream_t st) {
-  const Plan b = plan<KIND>(x.rows, w.rows, cdiv(a.kbytes, ROW_BYTES));
+  const int64_t size = a.out_type == IC_F32 ? 4 : 2;
+  const bool aligned = ((reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)(a.ldy * size)) & 31) == 0;
+  const Plan b = plan<KIND>(x.rows, w.rows, cdiv(a.kbytes, ROW_BYTES), aligned);
   a.swap = b.swap;
   const Operand &p = b.swap ? w : x, &q = b.swap ? x : w;
   switch (b.bn) {

@@ -8,9 +8,15 @@
 //
 // A row is spread over TPR threads, 16 consecutive columns ("a chunk") to a
 // lane, which is one nvfp4 block, half an mxfp4 block, and the unit of the
-// register Hadamard.  The row stays in registers from the load to the codes
-// (CH chunks per thread), so HBM sees each input once and each output once;
-// rows too long for that are read again for each reduction (CH = 0), from L2.
+// register Hadamard.  Chunks are held two at a time as fp32 pairs (chunk A in
+// the low halves, chunk B, TPR chunks on, in the high ones), so additions and
+// products of both are one packed .f32x2 instruction.  The row stays in
+// registers from the load to the codes (NP pairs per thread), so HBM sees each
+// input once and each output once; rows too long for that are read again for
+// each reduction (NP = 0), from L2.  These kernels are bound by instruction
+// issue, not by HBM: hence packed arithmetic, three-input maxima, and for
+// rotation groups of 256 a shared-memory transpose in place of the lane digits'
+// shuffles.
 // The sum of squares is held in 64 bits, so the norm does not depend on the
 // order of its sum and codes next to a rounding border are reproducible.
 #include <cuda_fp8.h>
@@ -93,15 +99,19 @@ __device__ __forceinline__ void store16(T* p, int64_t left, const float (&v)[16]
   }
 }
 
-// |x| as ordered bits: NaN above infinity above every finite value
-__device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-constexpr unsigned INF_BITS = 0x7f800000u;
+constexpr unsigned INF_BITS = 0x7f800000u;  // |x| as bits: NaN above infinity above every finite value
 
+// max(|a|, |b|, |c|), NaN if one is
+__device__ __forceinline__ float amax3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// bits of the largest magnitude of a chunk
 __device__ __forceinline__ unsigned amax16(const float (&v)[16]) {
-  unsigned m = 0;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) m = max(m, abs_bits(v[j]));
-  return m;
+  const float a = amax3(v[0], v[1], v[2]), b = amax3(v[3], v[4], v[5]), c = amax3(v[6], v[7], v[8]),
+              d = amax3(v[9], v[10], v[11]), e = amax3(v[12], v[13], v[14]);
+  return __float_as_uint(amax3(amax3(a, b, c), amax3(d, e, v[15]), 0.f));
 }
 
 // 8 fp32 values -> 8 E2M1 codes (round to nearest even, saturating), element 0 in the low nibble
@@ -123,6 +133,15 @@ __device__ __forceinline__ uint32_t to_e4m3(float x) {
 __device__ __forceinline__ float from_e4m3(uint32_t b) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
 }
+// four values, each x + (x < 0 ? -1/2 : 1/2) towards zero (rhaz, for magnitudes within int8 and a
+// half), saturated to int8 codes, value 0 in the low byte
+__device__ __forceinline__ uint32_t int8x4(float a, float b, float c, float d) {
+  auto r = [](float x) { return __float2int_rz(__fadd_rn(x, copysignf(0.5f, x))); };
+  uint32_t w;
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(w) : "r"(r(d)), "r"(r(c)));
+  asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %0;" : "+r"(w) : "r"(r(b)), "r"(r(a)));
+  return w;
+}
 
 // reductions over the TPR threads of a row (TPR a multiple of 32); `buf` holds
 // one value per warp of the CTA
@@ -140,6 +159,84 @@ __device__ __forceinline__ V row_reduce(V v, int tpr, V* buf, F op) {
   return v;
 }
 
+// ------------------------------------------------------------ packed Hadamard
+// The stages of hadamard_regs16 (same order, same fp32 operations) on pairs.
+__device__ __forceinline__ void h4_pair(f2& x0, f2& x1, f2& x2, f2& x3) {
+  const f2 p = add2(x0, x1), m = sub2(x0, x1), P = add2(x2, x3), M = sub2(x2, x3);
+  x0 = add2(p, M);
+  x1 = sub2(p, M);
+  x2 = add2(m, P);
+  x3 = sub2(P, m);
+}
+__device__ __forceinline__ void two_digits(f2 (&v)[16]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) h4_pair(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) h4_pair(v[q], v[4 + q], v[8 + q], v[12 + q]);
+}
+__device__ __forceinline__ f2 shfl2(f2 x, int m) {
+  return pk2(__shfl_xor_sync(0xffffffffu, lo2(x), m), __shfl_xor_sync(0xffffffffu, hi2(x), m));
+}
+
+constexpr int TEAM_BYTES = 16 * 136;  // 16 rows of 16 pairs, 8 bytes apart from a multiple of the banks
+
+// rot = 256: both lane digits after one transpose of the team's 16 x 16 pairs
+__device__ __forceinline__ void hadamard256(f2 (&v)[16], unsigned char* team, int l) {
+  two_digits(v);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) *reinterpret_cast<f2*>(team + l * 136 + e * 8) = v[e];
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] = *reinterpret_cast<const f2*>(team + e * 136 + l * 8);
+  two_digits(v);
+  const f2 scale = pk2(0.0625f, 0.0625f);
+#pragma unroll
+  for (int e = 0; e < 16; ++e) *reinterpret_cast<f2*>(team + e * 136 + l * 8) = mul2(v[e], scale);
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 16; ++e) v[e] = *reinterpret_cast<const f2*>(team + l * 136 + e * 8);
+  __syncwarp();
+}
+
+// other group sizes: lane digits by shuffles
+__device__ __forceinline__ void hadamard_pair(f2 (&v)[16], int rot, int l) {
+  const int L = rot / 16;
+  if (is_pow4(rot)) {
+    two_digits(v);
+    float scale = 0.25f;
+    for (int m = 1; m < L; m <<= 2) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        v[j] = add2(add2(v[j], shfl2(v[j], m)), sub2(shfl2(v[j], 2 * m), shfl2(v[j], 3 * m)));
+      scale *= 0.5f;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = mul2(v[j], pk2(scale, scale));
+  } else {
+#pragma unroll
+    for (int st = 1; st < 16; st <<= 1) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (j & st) continue;
+        const f2 a0 = v[j], a1 = v[j + st];
+        v[j] = add2(a0, a1);
+        v[j + st] = sub2(a0, a1);
+      }
+    }
+    for (int m = 1; m < L; m <<= 1) {
+      const bool upper = (l & m) != 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const f2 o = shfl2(v[j], m);
+        v[j] = upper ? sub2(o, v[j]) : add2(v[j], o);
+      }
+    }
+    const float c = (float)(1.0 / sqrt((double)rot));  // fp32(1/sqrt(n)), rotation.py:36
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = mul2(v[j], pk2(c, c));
+  }
+}
+
 // what the row's codes are formed with
 struct RowScale {
   float s;    // int8: reciprocal of the row's scale; nvfp4: g
@@ -147,50 +244,30 @@ struct RowScale {
   bool bad;   // a value of the row is not finite: codes 0
 };
 
+// The block scale of a chunk with largest magnitude m (bits): its byte, and what
+// the codes are multiplied with
 template <int FMT>
-__device__ __forceinline__ int emit_chunk(const RowArgs& a, int64_t row, int64_t c, int64_t nch, float (&v)[16],
-                                          const RowScale& rs) {
-  const int lane = threadIdx.x & 31;
-  const bool live = row < a.M && c < nch;
-  if (FMT == IC_INT8) {
-    uint32_t w[4];
-    int sum = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i] = 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const float y = rs.bad ? 0.f : rhaz(__fmul_rn(v[4 * i + u], rs.s));
-        const int code = (int)fminf(fmaxf(y, -128.f), 127.f);
-        sum += code;
-        w[i] |= (uint32_t)(code & 255) << (8 * u);
-      }
-    }
-    if (live) *reinterpret_cast<uint4*>(static_cast<int8_t*>(a.q) + row * a.ldq + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-    return live ? sum : 0;
-  }
-  uint32_t byte;
-  float inv;
-  bool bad;
-  unsigned m = amax16(v);
+__device__ __forceinline__ void block_scale(unsigned m, const RowScale& rs, uint32_t& byte, float& inv, bool& bad) {
   if (FMT == IC_MXFP4) {
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));  // the block is this chunk and its neighbour
     bad = m >= INF_BITS;
     const uint32_t e = m >> 23;
     byte = bad ? 255u : (e > 2 ? e - 2 : 0u);
-    inv = bad ? 0.f : __uint_as_float((254u - byte) << 23);
+    inv = __uint_as_float((254u - byte) << 23);  // bad: a subnormal, unused
   } else {
     bad = m >= INF_BITS || rs.bad;
     byte = bad ? (rs.bad ? 0u : 0x7fu) : to_e4m3(__fmul_rn(__uint_as_float(m), rs.i6g));
-    const float s = from_e4m3(byte);
-    inv = bad || byte == 0 ? 0.f : __fdiv_rn(1.f, __fmul_rn(s, rs.s));
+    inv = bad || byte == 0 ? 0.f : __frcp_rn(__fmul_rn(from_e4m3(byte), rs.s));
   }
-  float y[16];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) y[j] = bad ? 0.f : __fmul_rn(v[j], inv);
-  const uint2 codes = make_uint2(e2m1x8(y), e2m1x8(y + 8));
-  if (live) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.q) + row * a.ldq + c * 8) = codes;
-  // four blocks' bytes to one word
+}
+
+// codes of one chunk of scaled values, and the scale bytes of four blocks as one word
+template <int FMT>
+__device__ __forceinline__ void store_fp4(const RowArgs& a, int64_t row, int64_t c, int64_t nch, const float (&y)[16],
+                                          uint32_t byte, bool bad) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t keep = bad ? 0u : 0xffffffffu;
+  const uint2 codes = make_uint2(e2m1x8(y) & keep, e2m1x8(y + 8) & keep);
+  if (row < a.M && c < nch) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.q) + row * a.ldq + c * 8) = codes;
   uint32_t word;
   int64_t kt;
   bool first;
@@ -208,6 +285,56 @@ __device__ __forceinline__ int emit_chunk(const RowArgs& a, int64_t row, int64_t
     first = (lane & 3) == 0;
   }
   if (first && kt < a.ktiles) *reinterpret_cast<uint32_t*>(a.scales + scale_word(row, kt, a.ktiles)) = word;
+}
+
+// Codes of a pair of chunks (ca, cb) with largest magnitudes ma, mb; returns the sum of the int8 codes
+template <int FMT>
+__device__ __forceinline__ int emit_pair(const RowArgs& a, int64_t row, int64_t ca, int64_t cb, int64_t nch, f2 (&v)[16],
+                                         unsigned ma, unsigned mb, const RowScale& rs) {
+  float ya[16], yb[16];
+  if (FMT == IC_INT8) {
+    const f2 s = pk2(rs.s, rs.s);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const f2 y = mul2(v[j], s);
+      ya[j] = lo2(y), yb[j] = hi2(y);
+    }
+    int sum = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float* y = h ? yb : ya;
+      const int64_t c = h ? cb : ca;
+      uint32_t w[4];
+      int part = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = rs.bad ? 0u : int8x4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+        part = __dp4a((int)w[i], 0x01010101, part);
+      }
+      if (row < a.M && c < nch) {
+        *reinterpret_cast<uint4*>(static_cast<int8_t*>(a.q) + row * a.ldq + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        sum += part;
+      }
+    }
+    return sum;
+  }
+  if (FMT == IC_MXFP4) {  // a block is this chunk and the neighbouring lane's
+    ma = max(ma, __shfl_xor_sync(0xffffffffu, ma, 1));
+    mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
+  }
+  uint32_t ba, bb;
+  float ia, ib;
+  bool xa, xb;
+  block_scale<FMT>(ma, rs, ba, ia, xa);
+  block_scale<FMT>(mb, rs, bb, ib, xb);
+  const f2 inv = pk2(ia, ib);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const f2 y = mul2(v[j], inv);
+    ya[j] = lo2(y), yb[j] = hi2(y);
+  }
+  store_fp4<FMT>(a, row, ca, nch, ya, ba, xa);
+  store_fp4<FMT>(a, row, cb, nch, yb, bb, xb);
   return 0;
 }
 
@@ -225,92 +352,118 @@ __device__ __forceinline__ void load_chunk(const RowArgs& a, int64_t row, int64_
     if (write && left > 0) store16(static_cast<T*>(a.residual_out) + row * a.ldo + c * 16, left, v);
   }
 }
-
-template <bool NORM>
-__device__ __forceinline__ void finish_chunk(const RowArgs& a, int64_t c, float (&v)[16], float rstd, int l) {
-  if (NORM) {
-    float w[16];
-    load16_any(a.weight, a.wdtype, a.K - c * 16 > 0 ? c * 16 : 0, a.K - c * 16, w);
+template <typename T, bool NORM>
+__device__ __forceinline__ void load_pair(const RowArgs& a, int64_t row, int64_t ca, int64_t cb, f2 (&v)[16], bool write) {
+  float x[16], y[16];
+  load_chunk<T, NORM>(a, row, ca, x, write);
+  load_chunk<T, NORM>(a, row, cb, y, write);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = __fmul_rn(__fmul_rn(v[j], rstd), w[j]);
-  }
-  if (a.rot) hadamard_regs16(v, a.rot, l);
+  for (int j = 0; j < 16; ++j) v[j] = pk2(x[j], y[j]);
 }
 
-template <typename T, int FMT, bool NORM, int CH>
-__global__ void __launch_bounds__(512) rows_kernel(const RowArgs a) {
+template <bool NORM, bool T256>
+__device__ __forceinline__ void finish_pair(const RowArgs& a, int64_t ca, int64_t cb, f2 (&v)[16], float rstd,
+                                            unsigned char* team) {
+  if (NORM) {
+    float x[16], y[16];
+    load16_any(a.weight, a.wdtype, a.K - ca * 16 > 0 ? ca * 16 : 0, a.K - ca * 16, x);
+    load16_any(a.weight, a.wdtype, a.K - cb * 16 > 0 ? cb * 16 : 0, a.K - cb * 16, y);
+    const f2 r = pk2(rstd, rstd);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = mul2(mul2(v[j], r), pk2(x[j], y[j]));
+  }
+  if (T256) hadamard256(v, team, threadIdx.x & 15);
+  else if (a.rot) hadamard_pair(v, a.rot, threadIdx.x & (a.rot / 16 - 1));
+}
+__device__ __forceinline__ void amax_pair(const f2 (&v)[16], unsigned& ma, unsigned& mb) {
+  float x[16], y[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) x[j] = lo2(v[j]), y[j] = hi2(v[j]);
+  ma = amax16(x);
+  mb = amax16(y);
+}
+
+template <typename T, int FMT, bool NORM, int NP, bool T256>
+__global__ void __launch_bounds__(NP == 2 ? 512 : 256) rows_kernel(const RowArgs a) {
   __shared__ double buf[32];
+  extern __shared__ __align__(16) unsigned char teams[];  // T256: TEAM_BYTES for every 16 threads
+  unsigned char* team = teams + (threadIdx.x >> 4) * TEAM_BYTES;
   const int tpr = a.tpr, t = threadIdx.x & (tpr - 1);
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
   const int64_t nch = cdiv(a.kp, 16);
-  const int l = a.rot ? (threadIdx.x & (a.rot / 16 - 1)) : 0;  // this lane's chunk of its rotation group
-  const int n = CH ? CH : (int)cdiv(nch, tpr);
-  constexpr bool NEED_AMAX = FMT == IC_INT8 || FMT == IC_NVFP4;
-  float v[CH ? CH : 1][16];
+  const int n = NP ? NP : (int)cdiv(nch, 2 * tpr);
+  constexpr bool ROW = FMT != IC_MXFP4;  // the codes need the row's largest magnitude
+  constexpr int R = NP ? NP : 1;
+  f2 v[R][16];
+  unsigned ma[R], mb[R];
+  auto ca = [&](int i) { return (int64_t)(2 * i) * tpr + t; };
+  auto cb = [&](int i) { return (int64_t)(2 * i + 1) * tpr + t; };
   float rstd = 0.f;
-  if (CH) {
+  if (NP) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) load_chunk<T, NORM>(a, row, (int64_t)i * tpr + t, v[i], true);
+    for (int i = 0; i < NP; ++i) load_pair<T, NORM>(a, row, ca(i), cb(i), v[i], true);
   }
   if (NORM) {
     double ss = 0.0;
 #pragma unroll
     for (int i = 0; i < n; ++i) {
-      if (!CH) load_chunk<T, NORM>(a, row, (int64_t)i * tpr + t, v[0], true);
+      if (!NP) load_pair<T, NORM>(a, row, ca(i), cb(i), v[0], true);
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        const double d = v[CH ? i : 0][j];
-        ss = fma(d, d, ss);
+        const double x = lo2(v[NP ? i : 0][j]), y = hi2(v[NP ? i : 0][j]);
+        ss = fma(x, x, ss);
+        ss = fma(y, y, ss);
       }
     }
     ss = row_reduce(ss, tpr, buf, [](double p, double q) { return p + q; });
     // squares of fp32 values cannot overflow here: an infinite sum is an infinite input, which marks the whole row
     rstd = isfinite(ss) ? (float)(1.0 / sqrt(ss / (double)a.K + (double)a.eps)) : __int_as_float(0x7fc00000);
   }
-  if (CH) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) finish_chunk<NORM>(a, (int64_t)i * tpr + t, v[i], rstd, l);
-  }
   RowScale rs{0.f, 0.f, false};
-  if (NEED_AMAX) {
-    unsigned m = 0;
-    if (!a.row_scale_in) {
+  unsigned m = 0;
+  if (NP || (ROW && !a.row_scale_in)) {
 #pragma unroll
-      for (int i = 0; i < n; ++i) {
-        if (!CH) {
-          load_chunk<T, NORM>(a, row, (int64_t)i * tpr + t, v[0], false);
-          finish_chunk<NORM>(a, (int64_t)i * tpr + t, v[0], rstd, l);
-        }
-        m = max(m, amax16(v[CH ? i : 0]));
-      }
+    for (int i = 0; i < n; ++i) {
+      const int k = NP ? i : 0;
+      if (!NP) load_pair<T, NORM>(a, row, ca(i), cb(i), v[k], false);
+      finish_pair<NORM, T256>(a, ca(i), cb(i), v[k], rstd, team);
+      amax_pair(v[k], ma[k], mb[k]);
+      m = max(m, max(ma[k], mb[k]));
+    }
+  }
+  if (ROW) {
+    float s;
+    if (!a.row_scale_in) {
+      m = __reduce_max_sync(0xffffffffu, m);
       m = row_reduce(m, tpr, reinterpret_cast<unsigned*>(buf), [](unsigned p, unsigned q) { return max(p, q); });
     }
-    float s;
     if (FMT == IC_INT8) {
       rs.bad = m >= INF_BITS;
       s = fmaxf(__fmul_rn(__uint_as_float(m), (float)(1.0 / 127.0)), LOWP_SCALE_FLOOR);
-      rs.s = __fdiv_rn(1.f, s);
+      rs.s = __frcp_rn(s);
     } else {
       if (a.row_scale_in) {
         s = row < a.M ? a.row_scale_in[row * a.rs_stride] : 1.f;
-        rs.bad = !(s > 0.f) || abs_bits(s) >= INF_BITS;
+        rs.bad = !(s > 0.f) || __float_as_uint(s) >= INF_BITS;
       } else {
         rs.bad = m >= INF_BITS;
         s = fmaxf(__fmul_rn(__uint_as_float(m), (float)(1.0 / 2688.0)), LOWP_SCALE_FLOOR);
       }
       rs.s = s;
-      rs.i6g = __fdiv_rn(1.f, __fmul_rn(6.f, s));
+      rs.i6g = __frcp_rn(__fmul_rn(6.f, s));
     }
     if (t == 0 && row < a.M) a.row_scale[row] = rs.bad ? __uint_as_float(0x7fc00000u) : s;
   }
   int sum = 0;
 #pragma unroll
   for (int i = 0; i < n; ++i) {
-    if (!CH) {
-      load_chunk<T, NORM>(a, row, (int64_t)i * tpr + t, v[0], false);
-      finish_chunk<NORM>(a, (int64_t)i * tpr + t, v[0], rstd, l);
+    const int k = NP ? i : 0;
+    if (!NP) {
+      load_pair<T, NORM>(a, row, ca(i), cb(i), v[k], false);
+      finish_pair<NORM, T256>(a, ca(i), cb(i), v[k], rstd, team);
+      amax_pair(v[k], ma[k], mb[k]);
     }
-    sum += emit_chunk<FMT>(a, row, (int64_t)i * tpr + t, nch, v[CH ? i : 0], rs);
+    sum += emit_pair<FMT>(a, row, ca(i), cb(i), nch, v[k], ma[k], mb[k], rs);
   }
   if (FMT == IC_INT8 && a.sums) {
     sum = row_reduce(sum, tpr, reinterpret_cast<int*>(buf), [](int p, int q) { return p + q; });
@@ -318,30 +471,42 @@ __global__ void __launch_bounds__(512) rows_kernel(const RowArgs a) {
   }
 }
 
+template <typename T, int FMT, bool NORM, int NP, bool T256>
+int launch_np(const RowArgs& a, int64_t grid, int threads, cudaStream_t st) {
+  const int smem = T256 ? threads / 16 * TEAM_BYTES : 0;
+  if (T256 && threads > 256) {
+    static std::atomic<unsigned long long> done{0};
+    IC_TRY(once_per_device(done, [=] {
+      IC_CUDA(cudaFuncSetAttribute(rows_kernel<T, FMT, NORM, NP, T256>, cudaFuncAttributeMaxDynamicSharedMemorySize, 32 * TEAM_BYTES));
+      return (int)IC_OK;
+    }));
+  }
+  rows_kernel<T, FMT, NORM, NP, T256><<<(unsigned)grid, threads, smem, st>>>(a);
+  IC_CHECK_LAUNCH();
+  return IC_OK;
+}
+
 template <typename T, int FMT, bool NORM>
 int launch_rows(RowArgs a, cudaStream_t st) {
-  const int64_t nch = cdiv(a.kp, 16);
-  // one chunk per thread up to 256 threads, then more chunks per thread
+  const int64_t pairs = cdiv(cdiv(a.kp, 16), 2);
+  // one pair of chunks per thread up to 256 threads, then two, then 512 threads
   int tpr = 32;
-  while (tpr < 256 && tpr < nch) tpr *= 2;
-  int ch = (int)cdiv(nch, tpr);
-  if (ch > 4) {
+  while (tpr < 256 && tpr < pairs) tpr *= 2;
+  int np = (int)cdiv(pairs, tpr);
+  if (np > 2 && pairs <= 1024) {
     tpr = 512;
-    ch = (int)cdiv(nch, tpr);
+    np = 2;
   }
   a.tpr = tpr;
   const int threads = std::max(tpr, 128);
-  const int rpc = threads / tpr;
   // the 4-bit formats' scale tiles hold 128 rows: the grid covers the padding rows too
   const int64_t rows = FMT == IC_INT8 ? a.M : cdiv(a.M, 128) * 128;
-  const int64_t grid = cdiv(rows, rpc);
+  const int64_t grid = cdiv(rows, threads / tpr);
   if (grid > INT32_MAX) return fail(IC_ERR_UNSUPPORTED, "quantize: too many rows");
-  if (ch <= 1) rows_kernel<T, FMT, NORM, 1><<<(unsigned)grid, threads, 0, st>>>(a);
-  else if (ch <= 2) rows_kernel<T, FMT, NORM, 2><<<(unsigned)grid, threads, 0, st>>>(a);
-  else if (ch <= 4) rows_kernel<T, FMT, NORM, 4><<<(unsigned)grid, threads, 0, st>>>(a);
-  else rows_kernel<T, FMT, NORM, 0><<<(unsigned)grid, threads, 0, st>>>(a);
-  IC_CHECK_LAUNCH();
-  return IC_OK;
+  const bool t256 = a.rot == 256;
+  if (np == 1) return t256 ? launch_np<T, FMT, NORM, 1, true>(a, grid, threads, st) : launch_np<T, FMT, NORM, 1, false>(a, grid, threads, st);
+  if (np == 2) return t256 ? launch_np<T, FMT, NORM, 2, true>(a, grid, threads, st) : launch_np<T, FMT, NORM, 2, false>(a, grid, threads, st);
+  return t256 ? launch_np<T, FMT, NORM, 0, true>(a, grid, threads, st) : launch_np<T, FMT, NORM, 0, false>(a, grid, threads, st);
 }
 
 template <typename T>
@@ -382,20 +547,19 @@ int check_rows(const char* what, const RowArgs& a, int dtype, int fmt) {
 }
 
 // ---------------------------------------------------------------- dequantize
+// One chunk per thread; blockDim = (chunks of a row, rows), both powers of two.
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* __restrict__ q, int64_t ldq, int64_t M, int64_t kp,
                                                       const uint8_t* __restrict__ scales, int64_t ktiles,
                                                       const float* __restrict__ row_scale, T* __restrict__ out,
                                                       int64_t ldo) {
-  const int64_t nch = cdiv(kp, 16);
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t row = i / nch, c = i - row * nch;
-  if (row >= M) return;
+  const int c = blockIdx.y * blockDim.x + threadIdx.x;
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, left = kp - (int64_t)c * 16;
+  if (row >= M || left <= 0) return;
   float v[16];
   if (FMT == IC_INT8) {
     const float s = row_scale[row];
     const int8_t* p = reinterpret_cast<const int8_t*>(q) + row * ldq + c * 16;
-    const int64_t left = kp - c * 16;
     if (left >= 16 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
       const uint4 raw = *reinterpret_cast<const uint4*>(p);
       const int8_t* e = reinterpret_cast<const int8_t*>(&raw);
@@ -406,38 +570,48 @@ __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* __restrict_
       for (int j = 0; j < 16; ++j) v[j] = j < left ? __fmul_rn((float)p[j], s) : 0.f;
     }
   } else {
-    const int64_t b = FMT == IC_MXFP4 ? c >> 1 : c;
+    const int b = FMT == IC_MXFP4 ? c >> 1 : c;
     const uint32_t byte = scales[scale_word(row, b >> 2, ktiles) + (b & 3)];
     const float s = FMT == IC_MXFP4 ? (byte == 255u ? __uint_as_float(0x7fc00000u)
                                                     : __uint_as_float(byte ? byte << 23 : 0x00400000u))
                                     : from_e4m3(byte);
     const float g = FMT == IC_NVFP4 ? row_scale[row] : 1.f;
-    const uint2 raw = *reinterpret_cast<const uint2*>(q + row * ldq + c * 8);
-    const uint32_t w[2] = {raw.x, raw.y};
+    const uint2 raw = *reinterpret_cast<const uint2*>(q + row * ldq + (int64_t)c * 8);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint32_t code = (w[j >> 3] >> (4 * (j & 7))) & 15u;
-      const uint32_t e = (code >> 1) & 3u, f = code & 1u;
-      // E2M1: 0, 0.5 below 1, else (1 + f/2) 2^(e-1)
-      float x = e ? __uint_as_float(((126u + e) << 23) | (f << 22)) : (f ? 0.5f : 0.f);
-      x = code & 8u ? -x : x;
-      v[j] = __fmul_rn(x, s);
-      if (FMT == IC_NVFP4) v[j] = __fmul_rn(v[j], g);
+    for (int i = 0; i < 2; ++i) {
+      uint32_t h[4];  // two codes each as a pair of halves, exactly
+      asm("{\n .reg .b8 b0, b1, b2, b3;\n mov.b32 {b0, b1, b2, b3}, %4;\n"
+          " cvt.rn.f16x2.e2m1x2 %0, b0;\n cvt.rn.f16x2.e2m1x2 %1, b1;\n"
+          " cvt.rn.f16x2.e2m1x2 %2, b2;\n cvt.rn.f16x2.e2m1x2 %3, b3;\n}"
+          : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+          : "r"(i ? raw.y : raw.x));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+        f2 y = mul2(pk2(x.x, x.y), pk2(s, s));
+        if (FMT == IC_NVFP4) y = mul2(y, pk2(g, g));
+        v[i * 8 + j * 2] = lo2(y);
+        v[i * 8 + j * 2 + 1] = hi2(y);
+      }
     }
   }
-  store16(out + row * ldo + c * 16, kp - c * 16, v);
+  store16(out + row * ldo + (int64_t)c * 16, left, v);
 }
 
 template <int FMT>
 int launch_dequant(const void* q, int64_t ldq, int64_t M, int64_t kp, const uint8_t* scales, int64_t ktiles,
                    const float* row_scale, int dtype, void* out, int64_t ldo, cudaStream_t st) {
   const uint8_t* p = static_cast<const uint8_t*>(q);
-  const int64_t grid = cdiv(M * cdiv(kp, 16), 256);
-  if (grid > INT32_MAX) return fail(IC_ERR_UNSUPPORTED, "dequantize: too many elements");
+  const int64_t nch = cdiv(kp, 16);
+  int tx = 1;
+  while (tx < 256 && tx < nch) tx *= 2;
+  const dim3 block(tx, 256 / tx);
+  if (cdiv(nch, tx) > 65535 || cdiv(M, block.y) > INT32_MAX) return fail(IC_ERR_UNSUPPORTED, "dequantize: size");
+  const dim3 grid((unsigned)cdiv(M, block.y), (unsigned)cdiv(nch, tx));
   switch (dtype) {
-    case IC_F32: dequant_kernel<float, FMT><<<(unsigned)grid, 256, 0, st>>>(p, ldq, M, kp, scales, ktiles, row_scale, (float*)out, ldo); break;
-    case IC_F16: dequant_kernel<__half, FMT><<<(unsigned)grid, 256, 0, st>>>(p, ldq, M, kp, scales, ktiles, row_scale, (__half*)out, ldo); break;
-    case IC_BF16: dequant_kernel<__nv_bfloat16, FMT><<<(unsigned)grid, 256, 0, st>>>(p, ldq, M, kp, scales, ktiles, row_scale, (__nv_bfloat16*)out, ldo); break;
+    case IC_F32: dequant_kernel<float, FMT><<<grid, block, 0, st>>>(p, ldq, M, kp, scales, ktiles, row_scale, (float*)out, ldo); break;
+    case IC_F16: dequant_kernel<__half, FMT><<<grid, block, 0, st>>>(p, ldq, M, kp, scales, ktiles, row_scale, (__half*)out, ldo); break;
+    case IC_BF16: dequant_kernel<__nv_bfloat16, FMT><<<grid, block, 0, st>>>(p, ldq, M, kp, scales, ktiles, row_scale, (__nv_bfloat16*)out, ldo); break;
     default: return fail(IC_ERR_INVALID, "dequantize: unknown dtype %d", dtype);
   }
   IC_CHECK_LAUNCH();

@@ -101,9 +101,9 @@ class FP4Tensor:
 def empty_fp4(rows: int, columns: int, fmt: str, dev: torch.device, in_features: int | None = None, rot_size: int = 0,
               lead: tuple | None = None) -> FP4Tensor:
     """An FP4Tensor of uninitialised parts."""
-    return FP4Tensor(torch.empty((rows, columns // 2), dtype=torch.uint8, device=dev),
-                     torch.empty((-(-rows // 128), _ktiles(fmt, columns), 32, 4, 4), dtype=torch.uint8, device=dev),
-                     torch.empty((rows,), dtype=torch.float32, device=dev) if fmt == "nvfp4" else None, fmt, in_features,
+    return FP4Tensor(torch.empty(rows, columns // 2, dtype=torch.uint8, device=dev),
+                     torch.empty(-(-rows // 128), _ktiles(fmt, columns), 32, 4, 4, dtype=torch.uint8, device=dev),
+                     torch.empty(rows, dtype=torch.float32, device=dev) if fmt == "nvfp4" else None, fmt, in_features,
                      rot_size, lead)
 
 
@@ -180,11 +180,11 @@ def dequantize_fp4(q: FP4Tensor, dtype: torch.dtype = torch.float32) -> torch.Te
     dev = device_of(q.packed)
     d = q if q.packed.is_cuda else q.to(dev)
     rows, columns = d.rows, d.columns
-    out = torch.empty((rows, columns), dtype=dtype, device=dev)
+    out = torch.empty(rows, columns, dtype=dtype, device=dev)
     if rows and columns:
         call("ic_fp4_dequantize", dev, d.packed.data_ptr(), d.scales.data_ptr(), nat.ptr(d.row_scale), FORMATS[q.fmt], rows,
              columns, _DT[dtype], out.data_ptr(), columns)
-    if q.lead is not None:
+    if q.lead is not None and len(q.lead) != 1:
         out = out.reshape(*q.lead, columns)
     return back(out, q.packed)
 
@@ -226,7 +226,7 @@ def matmul_fp4(a: FP4Tensor, b: FP4Tensor, bias: torch.Tensor | None = None,
     dev = device_of(pa)
     bias_d = check_bias(bias, n, dev)
     da, db = (a, b) if pa.is_cuda else (a.to(dev), b.to(dev))
-    y = torch.empty((m, n), dtype=out_dtype, device=dev)
+    y = torch.empty(m, n, dtype=out_dtype, device=dev)
     if m and n:
         if half == 0:
             y.zero_() if bias_d is None else y.copy_(bias_d.float().expand(m, n))
@@ -234,6 +234,6 @@ def matmul_fp4(a: FP4Tensor, b: FP4Tensor, bias: torch.Tensor | None = None,
             call("ic_fp4_matmul", dev, da.packed.data_ptr(), da.scales.data_ptr(), nat.ptr(da.row_scale),
                  db.packed.data_ptr(), db.scales.data_ptr(), nat.ptr(db.row_scale), FORMATS[a.fmt], m, n, 2 * half,
                  nat.ptr(bias_d), 0 if bias_d is None else _DT[bias_d.dtype], _DT[out_dtype], y.data_ptr(), n)
-    if a.lead is not None:
+    if a.lead is not None and len(a.lead) != 1:
         y = y.reshape(*a.lead, n)
     return back(y, pa)

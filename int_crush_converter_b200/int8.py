@@ -61,9 +61,9 @@ class Int8Rows:
 def empty_int8(rows: int, columns: int, dev: torch.device, in_features: int | None = None, rot_size: int = 0,
                lead: tuple | None = None) -> Int8Rows:
     """Int8Rows of uninitialised parts, rows at a pitch of a multiple of 16 bytes."""
-    buf = torch.empty((rows, (columns + 15) & ~15), dtype=torch.int8, device=dev)
-    return Int8Rows(buf[:, :columns] if columns & 15 else buf, torch.empty((rows, 1), dtype=torch.float32, device=dev),
-                    torch.empty((rows,), dtype=torch.int32, device=dev), in_features, rot_size, lead)
+    buf = torch.empty(rows, (columns + 15) & ~15, dtype=torch.int8, device=dev)
+    return Int8Rows(buf[:, :columns] if columns & 15 else buf, torch.empty(rows, 1, dtype=torch.float32, device=dev),
+                    torch.empty(rows, dtype=torch.int32, device=dev), in_features, rot_size, lead)
 
 
 def flat(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
@@ -95,7 +95,7 @@ def dequantize_int8(q: Int8Rows, dtype: torch.dtype = torch.float32) -> torch.Te
         raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     dev = device_of(q.codes)
     rows, columns = q.codes.shape
-    out = torch.empty((rows, columns), dtype=dtype, device=dev)
+    out = torch.empty(rows, columns, dtype=dtype, device=dev)
     if rows and columns:
         codes = q.codes if q.codes.is_cuda else q.codes.to(dev)
         pitch, step = codes.stride()
@@ -104,7 +104,7 @@ def dequantize_int8(q: Int8Rows, dtype: torch.dtype = torch.float32) -> torch.Te
             pitch = columns
         call("ic_int8_dequantize", dev, codes.data_ptr(), pitch, flat(q.scales, dev).data_ptr(), rows, columns, _DT[dtype],
              out.data_ptr(), columns)
-    if q.lead is not None:
+    if q.lead is not None and len(q.lead) != 1:
         out = out.reshape(*q.lead, columns)
     return back(out, q.codes)
 
@@ -140,7 +140,7 @@ def matmul_int8(a: Int8Rows, w_codes: torch.Tensor, w_scales: torch.Tensor,
         raise ValueError("matmul_int8: operands are on different devices")
     dev = device_of(a.codes)
     bias_d = check_bias(bias, n, dev)
-    y = torch.empty((m, n), dtype=out_dtype, device=dev)
+    y = torch.empty(m, n, dtype=out_dtype, device=dev)
     if m and n:
         if k == 0:
             y.zero_() if bias_d is None else y.copy_(bias_d.float().expand(m, n))
@@ -159,6 +159,6 @@ def matmul_int8(a: Int8Rows, w_codes: torch.Tensor, w_scales: torch.Tensor,
             call("ic_int8_matmul", dev, x.data_ptr(), ldx, s.data_ptr(), nat.ptr(sums), w.data_ptr(), ldw, ws.data_ptr(),
                  nat.ptr(zp), m, n, k, nat.ptr(bias_d), 0 if bias_d is None else _DT[bias_d.dtype], _DT[out_dtype],
                  y.data_ptr(), n)
-    if a.lead is not None:
+    if a.lead is not None and len(a.lead) != 1:
         y = y.reshape(*a.lead, n)
     return back(y, a.codes)

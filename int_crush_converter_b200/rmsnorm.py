@@ -48,7 +48,7 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     r2 = None if residual is None else as_rows(residual, dev)
     w = weight if weight.is_cuda and weight.is_contiguous() else weight.to(dev).reshape(-1).contiguous()
     rows, kp = x2.shape[0], padded_columns(k, fmt, rot_size)
-    h = None if residual is None else torch.empty((rows, k), dtype=x.dtype, device=dev)
+    h = None if residual is None else torch.empty(rows, k, dtype=x.dtype, device=dev)
     if fmt == "int8":
         q = empty_int8(rows, kp, dev, k, rot_size, lead)
         codes, ldq, scales, row, sums = q.codes, (kp + 15) & ~15, None, q.scales, q.sums
@@ -64,4 +64,4 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
             q.codes, q.scales, q.sums = q.codes.to(x.device), q.scales.to(x.device), q.sums.to(x.device)
         else:
             q = q.to(x.device)
-    return q, None if h is None else back(h.view(x.shape), x)
+    return q, None if h is None else back(h if x.dim() == 2 else h.view(x.shape), x)
