@@ -46,7 +46,8 @@ struct RowArgs {
   int64_t ktiles;
   float* row_scale;
   int32_t* sums;
-  int tpr;
+  int tpr;         // threads per row
+  int64_t groups;  // row groups, blockDim.x / tpr rows each
 };
 
 // 16 elements from p; elements at or beyond `left` read as zero
@@ -338,40 +339,83 @@ __device__ __forceinline__ int emit_pair(const RowArgs& a, int64_t row, int64_t 
   return 0;
 }
 
-// h = x + residual of one chunk, optionally written to residual_out
-template <typename T, bool NORM>
-__device__ __forceinline__ void load_chunk(const RowArgs& a, int64_t row, int64_t c, float (&v)[16], bool write) {
-  const int64_t left = row < a.M ? a.K - c * 16 : 0;
-  load16(static_cast<const T*>(a.x) + (left > 0 ? row * a.ldx + c * 16 : 0), left, v);
-  if (NORM && a.residual) {
-    float r[16];
-    load16(static_cast<const T*>(a.residual) + (left > 0 ? row * a.ldr + c * 16 : 0), left, r);
+// 16 elements as loaded, converted when they are used: loads stay ahead of the
+// stores and reductions between them
+template <typename T>
+struct Raw {
+  static constexpr int V = 16 / sizeof(T);
+  uint4 r[16 / V];
+  // elements at or beyond `left` are zero
+  __device__ __forceinline__ void load(const T* p, int64_t left) {
+    if (left >= 16 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = __fadd_rn(v[j], r[j]);
-    // the stream's value is rounded to its type here; the norm goes on from the sum in 32 bits
-    if (write && left > 0) store16(static_cast<T*>(a.residual_out) + row * a.ldo + c * 16, left, v);
+      for (int i = 0; i < 16 / V; ++i) r[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16 / V; ++i) {
+        T e[V];
+#pragma unroll
+        for (int u = 0; u < V; ++u) e[u] = i * V + u < left ? p[i * V + u] : from_f32<T>(0.f);
+        r[i] = *reinterpret_cast<const uint4*>(e);
+      }
+    }
   }
-}
+  __device__ __forceinline__ float get(int j) const { return load_as_f32(reinterpret_cast<const T*>(&r[j / V]) + j % V); }
+};
+
+// the loads of a pair of chunks of one row
+template <typename T, bool NORM>
+struct RawPair {
+  Raw<T> x[2], r[2];
+  __device__ __forceinline__ void load(const RowArgs& a, int64_t row, int64_t ca, int64_t cb) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t c = h ? cb : ca, left = row < a.M ? a.K - c * 16 : 0;
+      x[h].load(static_cast<const T*>(a.x) + (left > 0 ? row * a.ldx + c * 16 : 0), left);
+      if (NORM && a.residual) r[h].load(static_cast<const T*>(a.residual) + (left > 0 ? row * a.ldr + c * 16 : 0), left);
+    }
+  }
+  // h = x + residual as pairs, optionally written to residual_out
+  __device__ __forceinline__ void add(const RowArgs& a, int64_t row, int64_t ca, int64_t cb, f2 (&v)[16], bool write) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = pk2(x[0].get(j), x[1].get(j));
+    if (NORM && a.residual) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = add2(v[j], pk2(r[0].get(j), r[1].get(j)));
+      // the stream's value is rounded to its type here; the norm goes on from the sum in 32 bits
+      if (write && row < a.M) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int64_t c = h ? cb : ca;
+          float y[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) y[j] = h ? hi2(v[j]) : lo2(v[j]);
+          if (a.K > c * 16) store16(static_cast<T*>(a.residual_out) + row * a.ldo + c * 16, a.K - c * 16, y);
+        }
+      }
+    }
+  }
+};
 template <typename T, bool NORM>
 __device__ __forceinline__ void load_pair(const RowArgs& a, int64_t row, int64_t ca, int64_t cb, f2 (&v)[16], bool write) {
-  float x[16], y[16];
-  load_chunk<T, NORM>(a, row, ca, x, write);
-  load_chunk<T, NORM>(a, row, cb, y, write);
-#pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = pk2(x[j], y[j]);
+  RawPair<T, NORM> p;
+  p.load(a, row, ca, cb);
+  p.add(a, row, ca, cb, v, write);
 }
 
-template <bool NORM, bool T256>
-__device__ __forceinline__ void finish_pair(const RowArgs& a, int64_t ca, int64_t cb, f2 (&v)[16], float rstd,
-                                            unsigned char* team) {
-  if (NORM) {
-    float x[16], y[16];
-    load16_any(a.weight, a.wdtype, a.K - ca * 16 > 0 ? ca * 16 : 0, a.K - ca * 16, x);
-    load16_any(a.weight, a.wdtype, a.K - cb * 16 > 0 ? cb * 16 : 0, a.K - cb * 16, y);
-    const f2 r = pk2(rstd, rstd);
+// (loading the weights ahead of the reduction as well took 126 instead of 80 registers and 47 instead of 39 us
+// for 4608 x 4096 int8)
+__device__ __forceinline__ void weigh_pair(const RowArgs& a, int64_t ca, int64_t cb, f2 (&v)[16], float rstd) {
+  float x[16], y[16];
+  load16_any(a.weight, a.wdtype, a.K - ca * 16 > 0 ? ca * 16 : 0, a.K - ca * 16, x);
+  load16_any(a.weight, a.wdtype, a.K - cb * 16 > 0 ? cb * 16 : 0, a.K - cb * 16, y);
+  const f2 r = pk2(rstd, rstd);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = mul2(mul2(v[j], r), pk2(x[j], y[j]));
-  }
+  for (int j = 0; j < 16; ++j) v[j] = mul2(mul2(v[j], r), pk2(x[j], y[j]));
+}
+
+template <bool T256>
+__device__ __forceinline__ void rotate_pair(const RowArgs& a, f2 (&v)[16], unsigned char* team) {
   if (T256) hadamard256(v, team, threadIdx.x & 15);
   else if (a.rot) hadamard_pair(v, a.rot, threadIdx.x & (a.rot / 16 - 1));
 }
@@ -383,105 +427,131 @@ __device__ __forceinline__ void amax_pair(const f2 (&v)[16], unsigned& ma, unsig
   mb = amax16(y);
 }
 
+// A CTA takes groups of rows by turns and loads the next group's while it works
+// on this one's (NP > 0): about a third of a row's time is otherwise spent
+// waiting for HBM between two barriers.
 template <typename T, int FMT, bool NORM, int NP, bool T256>
 __global__ void __launch_bounds__(NP == 2 ? 512 : 256) rows_kernel(const RowArgs a) {
   __shared__ double buf[32];
   extern __shared__ __align__(16) unsigned char teams[];  // T256: TEAM_BYTES for every 16 threads
   unsigned char* team = teams + (threadIdx.x >> 4) * TEAM_BYTES;
-  const int tpr = a.tpr, t = threadIdx.x & (tpr - 1);
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / tpr) + threadIdx.x / tpr;
+  const int tpr = a.tpr, t = threadIdx.x & (tpr - 1), rpc = blockDim.x / tpr;
   const int64_t nch = cdiv(a.kp, 16);
   const int n = NP ? NP : (int)cdiv(nch, 2 * tpr);
   constexpr bool ROW = FMT != IC_MXFP4;  // the codes need the row's largest magnitude
   constexpr int R = NP ? NP : 1;
-  f2 v[R][16];
-  unsigned ma[R], mb[R];
   auto ca = [&](int i) { return (int64_t)(2 * i) * tpr + t; };
   auto cb = [&](int i) { return (int64_t)(2 * i + 1) * tpr + t; };
-  float rstd = 0.f;
+  RawPair<T, NORM> raw[R];
+  int64_t row = (int64_t)blockIdx.x * rpc + threadIdx.x / tpr;
   if (NP) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) load_pair<T, NORM>(a, row, ca(i), cb(i), v[i], true);
+    for (int i = 0; i < R; ++i) raw[i].load(a, row, ca(i), cb(i));
   }
-  if (NORM) {
-    double ss = 0.0;
+  for (int64_t group = blockIdx.x; group < a.groups; group += gridDim.x, row += (int64_t)gridDim.x * rpc) {
+    f2 v[R][16];
+    unsigned ma[R], mb[R];
+    float rstd = 0.f;
+    if (NP) {
 #pragma unroll
-    for (int i = 0; i < n; ++i) {
-      if (!NP) load_pair<T, NORM>(a, row, ca(i), cb(i), v[0], true);
+      for (int i = 0; i < R; ++i) raw[i].add(a, row, ca(i), cb(i), v[i], true);
+      if (group + gridDim.x < a.groups) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const double x = lo2(v[NP ? i : 0][j]), y = hi2(v[NP ? i : 0][j]);
-        ss = fma(x, x, ss);
-        ss = fma(y, y, ss);
+        for (int i = 0; i < R; ++i) raw[i].load(a, row + (int64_t)gridDim.x * rpc, ca(i), cb(i));
       }
     }
-    ss = row_reduce(ss, tpr, buf, [](double p, double q) { return p + q; });
-    // squares of fp32 values cannot overflow here: an infinite sum is an infinite input, which marks the whole row
-    rstd = isfinite(ss) ? (float)(1.0 / sqrt(ss / (double)a.K + (double)a.eps)) : __int_as_float(0x7fc00000);
-  }
-  RowScale rs{0.f, 0.f, false};
-  unsigned m = 0;
-  if (NP || (ROW && !a.row_scale_in)) {
+    auto finish = [&](int i, int k) {
+      if (NORM) weigh_pair(a, ca(i), cb(i), v[k], rstd);
+      rotate_pair<T256>(a, v[k], team);
+      amax_pair(v[k], ma[k], mb[k]);
+    };
+    if (NORM) {
+      double ss = 0.0;
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        if (!NP) load_pair<T, NORM>(a, row, ca(i), cb(i), v[0], true);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const double x = lo2(v[NP ? i : 0][j]), y = hi2(v[NP ? i : 0][j]);
+          ss = fma(x, x, ss);
+          ss = fma(y, y, ss);
+        }
+      }
+      ss = row_reduce(ss, tpr, buf, [](double p, double q) { return p + q; });
+      // squares of fp32 values cannot overflow here: an infinite sum is an infinite input, which marks the whole row
+      rstd = isfinite(ss) ? (float)(1.0 / sqrt(ss / (double)a.K + (double)a.eps)) : __int_as_float(0x7fc00000);
+    }
+    RowScale rs{0.f, 0.f, false};
+    unsigned m = 0;
+    if (NP || (ROW && !a.row_scale_in)) {
+#pragma unroll
+      for (int i = 0; i < n; ++i) {
+        const int k = NP ? i : 0;
+        if (!NP) load_pair<T, NORM>(a, row, ca(i), cb(i), v[k], false);
+        finish(i, k);
+        m = max(m, max(ma[k], mb[k]));
+      }
+    }
+    if (ROW) {
+      float s;
+      if (!a.row_scale_in) {
+        m = __reduce_max_sync(0xffffffffu, m);
+        m = row_reduce(m, tpr, reinterpret_cast<unsigned*>(buf), [](unsigned p, unsigned q) { return max(p, q); });
+      }
+      if (FMT == IC_INT8) {
+        rs.bad = m >= INF_BITS;
+        s = fmaxf(__fmul_rn(__uint_as_float(m), (float)(1.0 / 127.0)), LOWP_SCALE_FLOOR);
+        rs.s = __frcp_rn(s);
+      } else {
+        if (a.row_scale_in) {
+          s = row < a.M ? a.row_scale_in[row * a.rs_stride] : 1.f;
+          rs.bad = !(s > 0.f) || __float_as_uint(s) >= INF_BITS;
+        } else {
+          rs.bad = m >= INF_BITS;
+          s = fmaxf(__fmul_rn(__uint_as_float(m), (float)(1.0 / 2688.0)), LOWP_SCALE_FLOOR);
+        }
+        rs.s = s;
+        rs.i6g = __frcp_rn(__fmul_rn(6.f, s));
+      }
+      if (t == 0 && row < a.M) a.row_scale[row] = rs.bad ? __uint_as_float(0x7fc00000u) : s;
+    }
+    int sum = 0;
 #pragma unroll
     for (int i = 0; i < n; ++i) {
       const int k = NP ? i : 0;
-      if (!NP) load_pair<T, NORM>(a, row, ca(i), cb(i), v[k], false);
-      finish_pair<NORM, T256>(a, ca(i), cb(i), v[k], rstd, team);
-      amax_pair(v[k], ma[k], mb[k]);
-      m = max(m, max(ma[k], mb[k]));
-    }
-  }
-  if (ROW) {
-    float s;
-    if (!a.row_scale_in) {
-      m = __reduce_max_sync(0xffffffffu, m);
-      m = row_reduce(m, tpr, reinterpret_cast<unsigned*>(buf), [](unsigned p, unsigned q) { return max(p, q); });
-    }
-    if (FMT == IC_INT8) {
-      rs.bad = m >= INF_BITS;
-      s = fmaxf(__fmul_rn(__uint_as_float(m), (float)(1.0 / 127.0)), LOWP_SCALE_FLOOR);
-      rs.s = __frcp_rn(s);
-    } else {
-      if (a.row_scale_in) {
-        s = row < a.M ? a.row_scale_in[row * a.rs_stride] : 1.f;
-        rs.bad = !(s > 0.f) || __float_as_uint(s) >= INF_BITS;
-      } else {
-        rs.bad = m >= INF_BITS;
-        s = fmaxf(__fmul_rn(__uint_as_float(m), (float)(1.0 / 2688.0)), LOWP_SCALE_FLOOR);
+      if (!NP) {
+        load_pair<T, NORM>(a, row, ca(i), cb(i), v[k], false);
+        finish(i, k);
       }
-      rs.s = s;
-      rs.i6g = __frcp_rn(__fmul_rn(6.f, s));
+      sum += emit_pair<FMT>(a, row, ca(i), cb(i), nch, v[k], ma[k], mb[k], rs);
     }
-    if (t == 0 && row < a.M) a.row_scale[row] = rs.bad ? __uint_as_float(0x7fc00000u) : s;
-  }
-  int sum = 0;
-#pragma unroll
-  for (int i = 0; i < n; ++i) {
-    const int k = NP ? i : 0;
-    if (!NP) {
-      load_pair<T, NORM>(a, row, ca(i), cb(i), v[k], false);
-      finish_pair<NORM, T256>(a, ca(i), cb(i), v[k], rstd, team);
-      amax_pair(v[k], ma[k], mb[k]);
+    if (FMT == IC_INT8 && a.sums) {
+      sum = row_reduce(sum, tpr, reinterpret_cast<int*>(buf), [](int p, int q) { return p + q; });
+      if (t == 0 && row < a.M) a.sums[row] = sum;
     }
-    sum += emit_pair<FMT>(a, row, ca(i), cb(i), nch, v[k], ma[k], mb[k], rs);
-  }
-  if (FMT == IC_INT8 && a.sums) {
-    sum = row_reduce(sum, tpr, reinterpret_cast<int*>(buf), [](int p, int q) { return p + q; });
-    if (t == 0 && row < a.M) a.sums[row] = sum;
   }
 }
 
 template <typename T, int FMT, bool NORM, int NP, bool T256>
-int launch_np(const RowArgs& a, int64_t grid, int threads, cudaStream_t st) {
+int launch_np(const RowArgs& a, int threads, cudaStream_t st) {
+  const auto kernel = rows_kernel<T, FMT, NORM, NP, T256>;
   const int smem = T256 ? threads / 16 * TEAM_BYTES : 0;
-  if (T256 && threads > 256) {
-    static std::atomic<unsigned long long> done{0};
-    IC_TRY(once_per_device(done, [=] {
-      IC_CUDA(cudaFuncSetAttribute(rows_kernel<T, FMT, NORM, NP, T256>, cudaFuncAttributeMaxDynamicSharedMemorySize, 32 * TEAM_BYTES));
-      return (int)IC_OK;
-    }));
+  // CTAs that the device holds at once, by device and block size (128, 256 or 512 threads)
+  static std::atomic<int> resident[64][3];
+  int dev = 0;
+  IC_CUDA(cudaGetDevice(&dev));
+  std::atomic<int>& r = resident[dev & 63][threads == 128 ? 0 : threads == 256 ? 1 : 2];
+  int ctas = r.load();
+  if (!ctas) {
+    int sms = 0;
+    if (smem > 48 << 10) IC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    IC_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, threads, smem));
+    IC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    ctas = std::max(1, ctas) * sms;
+    r.store(ctas);
   }
-  rows_kernel<T, FMT, NORM, NP, T256><<<(unsigned)grid, threads, smem, st>>>(a);
+  const int64_t grid = NP ? std::min<int64_t>(a.groups, ctas) : a.groups;
+  kernel<<<(unsigned)grid, threads, smem, st>>>(a);
   IC_CHECK_LAUNCH();
   return IC_OK;
 }
@@ -501,12 +571,12 @@ int launch_rows(RowArgs a, cudaStream_t st) {
   const int threads = std::max(tpr, 128);
   // the 4-bit formats' scale tiles hold 128 rows: the grid covers the padding rows too
   const int64_t rows = FMT == IC_INT8 ? a.M : cdiv(a.M, 128) * 128;
-  const int64_t grid = cdiv(rows, threads / tpr);
-  if (grid > INT32_MAX) return fail(IC_ERR_UNSUPPORTED, "quantize: too many rows");
+  a.groups = cdiv(rows, threads / tpr);
+  if (a.groups > INT32_MAX) return fail(IC_ERR_UNSUPPORTED, "quantize: too many rows");
   const bool t256 = a.rot == 256;
-  if (np == 1) return t256 ? launch_np<T, FMT, NORM, 1, true>(a, grid, threads, st) : launch_np<T, FMT, NORM, 1, false>(a, grid, threads, st);
-  if (np == 2) return t256 ? launch_np<T, FMT, NORM, 2, true>(a, grid, threads, st) : launch_np<T, FMT, NORM, 2, false>(a, grid, threads, st);
-  return t256 ? launch_np<T, FMT, NORM, 0, true>(a, grid, threads, st) : launch_np<T, FMT, NORM, 0, false>(a, grid, threads, st);
+  if (np == 1) return t256 ? launch_np<T, FMT, NORM, 1, true>(a, threads, st) : launch_np<T, FMT, NORM, 1, false>(a, threads, st);
+  if (np == 2) return t256 ? launch_np<T, FMT, NORM, 2, true>(a, threads, st) : launch_np<T, FMT, NORM, 2, false>(a, threads, st);
+  return t256 ? launch_np<T, FMT, NORM, 0, true>(a, threads, st) : launch_np<T, FMT, NORM, 0, false>(a, threads, st);
 }
 
 template <typename T>
