@@ -81,10 +81,33 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// whole 32-byte sectors per lane
+__device__ __forceinline__ void load32(const void* p, uint4& a, uint4& b) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void store32(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w),
+               "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
 template <typename T>
 __device__ __forceinline__ void store16(T* p, int64_t left, const float (&v)[16]) {
   constexpr int V = 16 / sizeof(T);
-  if (left >= 16 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+  if (left >= 16 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+    uint4 raw[16 / V];
+#pragma unroll
+    for (int i = 0; i < 16 / V; ++i) {
+      T* e = reinterpret_cast<T*>(&raw[i]);
+#pragma unroll
+      for (int u = 0; u < V; ++u) e[u] = from_f32<T>(v[i * V + u]);
+    }
+#pragma unroll
+    for (int i = 0; i < 16 / V; i += 2) store32(p + i * V, raw[i], raw[i + 1]);
+  } else if (left >= 16 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
 #pragma unroll
     for (int i = 0; i < 16 / V; ++i) {
       uint4 raw;
@@ -206,9 +229,12 @@ __device__ __forceinline__ void hadamard_pair(f2 (&v)[16], int rot, int l) {
     two_digits(v);
     float scale = 0.25f;
     for (int m = 1; m < L; m <<= 2) {
+      // output k is (a_k + a_{k^1}) + (a_{k^2} - a_{k^3}): the difference comes whole from lane k^2
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        v[j] = add2(add2(v[j], shfl2(v[j], m)), sub2(shfl2(v[j], 2 * m), shfl2(v[j], 3 * m)));
+      for (int j = 0; j < 16; ++j) {
+        const f2 o = shfl2(v[j], m);
+        v[j] = add2(add2(v[j], o), shfl2(sub2(v[j], o), 2 * m));
+      }
       scale *= 0.5f;
     }
 #pragma unroll
@@ -225,12 +251,11 @@ __device__ __forceinline__ void hadamard_pair(f2 (&v)[16], int rot, int l) {
       }
     }
     for (int m = 1; m < L; m <<= 1) {
-      const bool upper = (l & m) != 0;
+      // the lower lane takes a + b, the upper a - b: its own value times 1 or -1, exactly, plus the other's
+      const float sign = (l & m) != 0 ? -1.f : 1.f;
+      const f2 own = pk2(sign, sign);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const f2 o = shfl2(v[j], m);
-        v[j] = upper ? sub2(o, v[j]) : add2(v[j], o);
-      }
+      for (int j = 0; j < 16; ++j) v[j] = fma2(v[j], own, shfl2(v[j], m));
     }
     const float c = (float)(1.0 / sqrt((double)rot));  // fp32(1/sqrt(n)), rotation.py:36
 #pragma unroll
@@ -347,7 +372,10 @@ struct Raw {
   uint4 r[16 / V];
   // elements at or beyond `left` are zero
   __device__ __forceinline__ void load(const T* p, int64_t left) {
-    if (left >= 16 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    if (left >= 16 && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+#pragma unroll
+      for (int i = 0; i < 16 / V; i += 2) load32(p + i * V, r[i], r[i + 1]);
+    } else if (left >= 16 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
 #pragma unroll
       for (int i = 0; i < 16 / V; ++i) r[i] = reinterpret_cast<const uint4*>(p)[i];
     } else {
