@@ -438,8 +438,13 @@ __device__ __forceinline__ void weigh_pair(const RowArgs& a, int64_t ca, int64_t
   load16_any(a.weight, a.wdtype, a.K - ca * 16 > 0 ? ca * 16 : 0, a.K - ca * 16, x);
   load16_any(a.weight, a.wdtype, a.K - cb * 16 > 0 ? cb * 16 : 0, a.K - cb * 16, y);
   const f2 r = pk2(rstd, rstd);
+  // the last product is a scalar one: ptxas merges a packed product with the rotation's additions into
+  // fused multiply-adds, which round differently from the product alone
 #pragma unroll
-  for (int j = 0; j < 16; ++j) v[j] = mul2(mul2(v[j], r), pk2(x[j], y[j]));
+  for (int j = 0; j < 16; ++j) {
+    const f2 h = mul2(v[j], r);
+    v[j] = pk2(__fmul_rn(lo2(h), x[j]), __fmul_rn(hi2(h), y[j]));
+  }
 }
 
 template <bool T256>

@@ -237,6 +237,19 @@ def test_rmsnorm_quantize(fmt, m, k, rot, dtype, wdtype, res):
     assert torch.equal(B.dequantize_int8(q, torch.bfloat16), want)
 
 
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("rot", [0, 16, 32, 64, 128, 256, 512])
+def test_rmsnorm_rounds_each_step(fmt, rot):
+    """The norm's fp32 products, rounded one by one, are what is rotated and quantized: bit for bit the
+    quantizer's own result on them (the norm itself in 64 bits, rounded to fp32)."""
+    x, r = rows(rot + 1, 200, 1100, torch.bfloat16), rows(rot + 2, 200, 1100, torch.bfloat16)
+    w = 1 + 0.3 * torch.randn(1100, device="cuda", generator=gen(4))
+    q, _ = B.rmsnorm_quantize(x, w, residual=r, eps=1e-5, fmt=fmt, rot_size=rot)
+    h = x.float() + r.float()
+    rstd = (1.0 / torch.sqrt((h.double() ** 2).mean(1, keepdim=True) + float(np.float32(1e-5)))).float()
+    assert same(q, B.quantize_fp4(h * rstd * w, fmt, rot_size=rot))
+
+
 def test_rmsnorm_int8_rounds_half_away():
     """Ties go away from zero, as in the framework's other INT8 codes.  The squares sum to
     16 * 32^2 and the largest value is 127, so that norm and scale are exact."""
