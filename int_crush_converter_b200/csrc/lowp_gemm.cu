@@ -245,6 +245,35 @@ __device__ __forceinline__ void store_vec(T* to, const T (&e)[V]) {
     *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(e);
 }
 
+// A warp's 32 rows of C columns through its shared memory `mine` (68 bytes a
+// row: the banks stay apart) to rows of y that are not 16-byte aligned:
+// neighbouring lanes store neighbouring elements.  v: this lane's row.
+constexpr int ROW_PITCH = 68;
+template <typename T, int C>
+__device__ __forceinline__ void store_rows(unsigned char* mine, const float (&v)[C], int rows, int cols, T* to, long long ld,
+                                           int lane) {
+  static_assert(C * sizeof(T) <= 64 && 32 % C == 0, "a row of the buffer");
+  uint32_t* w = reinterpret_cast<uint32_t*>(mine + lane * ROW_PITCH);
+#pragma unroll
+  for (int j = 0; j < C * (int)sizeof(T) / 4; ++j) {
+    if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(v[j]);
+    else {
+      T e[2] = {to_out<T>(v[2 * j]), to_out<T>(v[2 * j + 1])};
+      w[j] = *reinterpret_cast<const uint32_t*>(e);
+    }
+  }
+  __syncwarp();
+  constexpr int R = 32 / C;  // rows at a time
+  const int i = lane % C;
+#pragma unroll 8
+  for (int k = 0; k < 32; k += R) {
+    const int r = k + lane / C;
+    const T x = reinterpret_cast<const T*>(mine + r * ROW_PITCH)[i];
+    if (r < rows && i < cols) to[r * ld + i] = x;
+  }
+  __syncwarp();
+}
+
 // factors of a tile's rows and columns, by 128 threads
 template <int BN>
 __device__ __forceinline__ void load_factors(const LowpArgs& a, TileFactors& f, int p0, int q0, int t) {
@@ -336,7 +365,8 @@ __device__ __forceinline__ void epilogue(const LowpArgs& a, const TileFactors& f
     const float rowf = f.rowf[lr], rowb = f.rowb[lr];
     const int rowi = f.rowi[lr];
     constexpr int V = 32 / sizeof(T);
-    const bool vec = !a.swap && ((reinterpret_cast<uintptr_t>(y) | (uintptr_t)(a.ldy * (long long)sizeof(T))) & 31) == 0;
+    const uintptr_t at_y = reinterpret_cast<uintptr_t>(y) | (uintptr_t)(a.ldy * (long long)sizeof(T));
+    const bool vec = !a.swap && (at_y & 15) == 0, whole = (at_y & 31) == 0;
     const int cols = min(BN, a.qn - q0);
     for (int c = 0; c < cols; c += W) {
       uint32_t r[W];
@@ -371,22 +401,27 @@ __device__ __forceinline__ void epilogue(const LowpArgs& a, const TileFactors& f
           alignas(32) T e[V];
 #pragma unroll
           for (int u = 0; u < V; ++u) e[u] = to_out<T>(v[j + u]);
-          if (j + V <= left) store_vec<T, V>(to + j, e);
-          else
+          if (j + V <= left && whole) {
+            store_vec<T, V>(to + j, e);
+          } else if (j + V <= left) {
+            *reinterpret_cast<uint4*>(to + j) = *reinterpret_cast<const uint4*>(e);
+            *reinterpret_cast<uint4*>(to + j + V / 2) = *reinterpret_cast<const uint4*>(e + V / 2);
+          } else
 #pragma unroll
             for (int u = 0; u < V; ++u)
               if (j + u < left) to[j + u] = e[u];
         }
       } else {
-        // the stages are idle by now; 33 elements to a row keep the banks apart
-        T* mine = reinterpret_cast<T*>(smem) + q * (32 * 34);
+        unsigned char* mine = smem + q * (32 * ROW_PITCH);  // the stages are idle by now
+        constexpr int C = 64 / sizeof(T) < W ? 64 / sizeof(T) : W;
 #pragma unroll
-        for (int j = 0; j < W; ++j) mine[lane * 34 + j] = to_out<T>(v[j]);
-        __syncwarp();
-        const int rows = min(32, a.pm - p0 - q * 32), wide = min(W, cols - c);
-        if (lane < wide)
-          for (int i = 0; i < rows; ++i) y[(long long)(p0 + q * 32 + i) * a.ldy + q0 + c + lane] = mine[i * 34 + lane];
-        __syncwarp();
+        for (int g = 0; g < W; g += C) {
+          float part_v[C];
+#pragma unroll
+          for (int u = 0; u < C; ++u) part_v[u] = v[g + u];
+          store_rows<T, C>(mine, part_v, min(32, a.pm - p0 - q * 32), min(C, cols - c - g),
+                           y + (long long)(p0 + q * 32) * a.ldy + q0 + c + g, a.ldy, lane);
+        }
       }
     }
   }
@@ -565,7 +600,7 @@ struct PairCfg {
   static constexpr int SF_COLS = SF_TILES * 12;
   static constexpr int NACC = FP4 ? 1 : 2;
   static constexpr int TMEM_COLS = 512;
-  static constexpr int OUT_BYTES = 8 * 2048;  // per epilogue warp: 32 rows of 64 bytes
+  static constexpr int OUT_BYTES = 8 * 32 * ROW_PITCH;  // per epilogue warp: 32 rows of 64 bytes
   static constexpr int SMEM = STAGES * STAGE_BYTES + OUT_BYTES + 2 * (int)sizeof(Factors) + 1024 + 256;
   static_assert(NACC * BN + STAGES * SF_COLS <= TMEM_COLS, "tensor memory");
   static_assert(SMEM <= 232448, "shared memory");
@@ -644,18 +679,20 @@ __device__ __forceinline__ void finish4(const LowpArgs& a, const uint32_t* acc, 
 }
 
 // One warp's 32 rows x 128 columns of sums, from column c0 of the tile, to y.
-// Rows that are 32-byte aligned: each lane stores its own row in whole 32-byte
-// sectors, past shared memory, whose bandwidth the loads and products of the
-// next tile take up.  Other rows: through the warp's 2 KB `out`, 64 bytes of
-// each row at a time, so that neighbouring lanes store neighbouring elements.
+// Rows that are 32-byte (16-byte) aligned: each lane stores its own row in whole
+// (half) sectors, past shared memory, whose bandwidth the loads and products of the
+// next tile take up.  Other rows: through the warp's part `out` of it, 64 bytes
+// of each row at a time.
 template <int KIND, typename T>
 __device__ __forceinline__ void store_block(const LowpArgs& a, const uint32_t (&acc)[128], unsigned char* out,
                                             const Factors& f, int r0, int c0, int row0, int col0, int lane) {
   T* y = static_cast<T*>(a.y);
   const float rowf = f.row[r0 + lane];
   const int sum = f.sum[r0 + lane];
-  if (((reinterpret_cast<uintptr_t>(y) | (uintptr_t)(a.ldy * (long long)sizeof(T))) & 31) == 0) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(y) | (uintptr_t)(a.ldy * (long long)sizeof(T));
+  if ((at & 15) == 0) {
     constexpr int V = 32 / sizeof(T);
+    const bool whole = (at & 31) == 0;
     T* to = y + (long long)(row0 + lane) * a.ldy + col0;
     const int left = row0 + lane < a.pm ? a.qn - col0 : 0;
 #pragma unroll
@@ -668,8 +705,11 @@ __device__ __forceinline__ void store_block(const LowpArgs& a, const uint32_t (&
 #pragma unroll
         for (int w = 0; w < 4; ++w) e[u + w] = to_out<T>(v[w]);
       }
-      if (c + V <= left) {
+      if (c + V <= left && whole) {
         store_vec<T, V>(to + c, e);
+      } else if (c + V <= left) {
+        *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(e);
+        *reinterpret_cast<uint4*>(to + c + V / 2) = *reinterpret_cast<const uint4*>(e + V / 2);
       } else {
 #pragma unroll
         for (int u = 0; u < V; ++u)
@@ -678,32 +718,18 @@ __device__ __forceinline__ void store_block(const LowpArgs& a, const uint32_t (&
     }
     return;
   }
-  constexpr int G = 64 / sizeof(T);  // columns per pass
-  constexpr int V = 16 / sizeof(T);
+  constexpr int G = 64 / sizeof(T);  // columns at a time
 #pragma unroll
-  for (int g = 0; g < 128 / G; ++g) {
+  for (int g = 0; g < 128; g += G) {
+    float v[G];
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      alignas(16) T e[V];
+    for (int u = 0; u < G; u += 4) {
+      float x[4];
+      finish4<KIND>(a, acc + g + u, f, c0 + g + u, rowf, sum, x);
 #pragma unroll
-      for (int u = 0; u < V; u += 4) {
-        const int c = g * G + p * V + u;
-        float v[4];
-        finish4<KIND>(a, acc + c, f, c0 + c, rowf, sum, v);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) e[u + w] = to_out<T>(v[w]);
-      }
-      *reinterpret_cast<uint4*>(out + lane * 64 + ((p ^ ((lane >> 1) & 3)) << 4)) = *reinterpret_cast<const uint4*>(e);
+      for (int w = 0; w < 4; ++w) v[u + w] = x[w];
     }
-    __syncwarp();
-    const int rows = min(32, a.pm - row0), cols = min(G, a.qn - col0 - g * G);
-    for (int i = lane; i < rows * G; i += 32) {
-      const int r = i / G, c = i % G;
-      if (c < cols)
-        y[(long long)(row0 + r) * a.ldy + col0 + g * G + c] =
-            *reinterpret_cast<const T*>(out + r * 64 + (((c / V) ^ ((r >> 1) & 3)) << 4) + (c % V) * sizeof(T));
-    }
-    __syncwarp();
+    store_rows<T, G>(out, v, min(32, a.pm - row0), min(G, a.qn - col0 - g), y + (long long)row0 * a.ldy + col0 + g, a.ldy, lane);
   }
 }
 
@@ -880,7 +906,7 @@ __global__ void __launch_bounds__(384, 1)
   } else if (warp >= 4) {
     // ---------------- epilogue (both CTAs, own rows) ----------------
     const int q = warp & 3, h = (warp - 4) >> 2;
-    unsigned char* out = out_smem + (warp - 4) * 2048;
+    unsigned char* out = out_smem + (warp - 4) * (32 * ROW_PITCH);
     int t = 0;
     for (int tile = pair; tile < tiles; tile += pairs, ++t) {
       int p0, q0;
@@ -1070,10 +1096,10 @@ struct Plan {
 // Estimated SM clocks of a one-CTA plan.  A stage takes the longer of its
 // products (BN/2 clocks for each of four) and its loads (63 bytes a clock and
 // SM, measured with all SMs loading from L2); a CTA's start, first loads and
-// epilogue take about 4000 clocks and 8 a column, a split's exchange 2500 and 12
-// a column, element stores into rows that are not 32-byte aligned 20 a column.
-// (Over 24 products from 1 x 4096 x 4096 to 2048 x 12288 x 4096, every plan
-// timed: the choice is within 10% of the fastest.)
+// epilogue take about 4000 clocks and per column 8 (aligned rows of y), 45 (other
+// rows) or 20 (weights in P), a split's exchange 2500 and 16 a column.
+// (Over 24 products from 1 x 4096 x 4096 to 4607 x 16383 x 4096, every plan
+// timed: 21 choices are within 7% of the fastest, the worst 21% off.)
 template <int KIND, int BN>
 void consider(Plan& best, int64_t pm, int64_t qn, int64_t stages, bool swap, bool aligned) {
   using C = Cfg<KIND, BN>;
@@ -1082,8 +1108,8 @@ void consider(Plan& best, int64_t pm, int64_t qn, int64_t stages, bool swap, boo
     const int64_t ctas = tiles * s, waves = cdiv(ctas, 148 * C::CTAS);
     const int per_sm = (int)std::min<int64_t>(C::CTAS, cdiv(ctas, 148));
     const double stage = std::max(2.0 * BN, C::STAGE_BYTES / 63.0) * per_sm;
-    const double ends = 4000 + 8.0 * BN + (s > 1 ? 2500 + 12.0 * BN : 0) + (swap || aligned ? 0 : 20.0 * BN / s);
-    const double clocks = waves * ((double)cdiv(stages, s) * stage + ends);
+    const double store = swap ? 20 : aligned ? 8 : 45, ends = 4000 + store * BN / s + (s > 1 ? 2500 + 16.0 * BN : 0);
+    const double clocks = waves * ((double)cdiv(stages, s) * stage + ends * (per_sm > 1 ? 1.5 : 1));  // two CTAs share an SM's ends too
     if (clocks < best.clocks) best = Plan{BN, swap, s, clocks};
   }
 }
@@ -1091,7 +1117,7 @@ void consider(Plan& best, int64_t pm, int64_t qn, int64_t stages, bool swap, boo
 template <int KIND>
 Plan plan(int64_t m, int64_t n, int64_t stages, bool aligned) {
   // pairs: 620 clocks a stage and 3000 between tiles, or an epilogue of element stores; a longer start (measured)
-  Plan best{0, false, 1, cdiv(cdiv(m, 256) * cdiv(n, 256), 74) * std::max(stages * 620.0 + 3000, aligned ? 0.0 : 25000.0) + 5000};
+  Plan best{0, false, 1, cdiv(cdiv(m, 256) * cdiv(n, 256), 74) * std::max(stages * 620.0 + 3000, aligned ? 0.0 : 18000.0) + 5000};
   for (int swap = 0; swap < 2; ++swap) {
     const int64_t pm = swap ? n : m, qn = swap ? m : n;
     if (qn <= 16) consider<KIND, 16>(best, pm, qn, stages, swap, aligned);
@@ -1108,7 +1134,7 @@ Plan plan(int64_t m, int64_t n, int64_t stages, bool aligned) {
 template <int KIND>
 int matmul(const Operand& x, const Operand& w, LowpArgs a, cudaStream_t st) {
   const int64_t size = a.out_type == IC_F32 ? 4 : 2;
-  const bool aligned = ((reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)(a.ldy * size)) & 31) == 0;
+  const bool aligned = ((reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)(a.ldy * size)) & 15) == 0;
   const Plan b = plan<KIND>(x.rows, w.rows, cdiv(a.kbytes, ROW_BYTES), aligned);
   a.swap = b.swap;
   const Operand &p = b.swap ? w : x, &q = b.swap ? x : w;
