@@ -1160,6 +1160,22 @@ int check_product(const char* what, int64_t m, int64_t n, int64_t k, const void*
 }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// The device status word.  Where none exists yet it is this file's own static
+// one: allocating it would end a stream capture that the first product is part of.
+__device__ unsigned g_lowp_flags;
+unsigned* status_word() {
+  static std::atomic<unsigned long long> done{0};
+  const int r = once_per_device(done, [] {
+    int dev = 0;
+    void* p = nullptr;
+    IC_CUDA(cudaGetDevice(&dev));
+    IC_CUDA(cudaGetSymbolAddress(&p, g_lowp_flags));
+    register_device_flags(dev, static_cast<unsigned*>(p));
+    return (int)IC_OK;
+  });
+  return r == IC_OK ? device_flags() : nullptr;
+}
+
 }  // namespace
 }  // namespace ic
 
@@ -1180,7 +1196,7 @@ extern "C" int ic_fp4_matmul(const uint8_t* a_packed, const uint8_t* a_scales, c
   a.kbytes = (int)(kp / 2);
   a.ktiles = (int)fp4_ktiles(fmt, kp);
   a.bias = bias, a.bias_type = bias_dtype, a.y = y, a.ldy = ldy, a.out_type = out_dtype;
-  a.flags = device_flags();
+  a.flags = status_word();
   if (!a.flags) return fail(IC_ERR_CUDA, "device status word unavailable");
   const bool nv = fmt == IC_NVFP4;
   const Operand x{a_packed, m, kp / 2, a_scales, nv ? a_row_scale : nullptr, 0};
@@ -1204,7 +1220,7 @@ extern "C" int ic_int8_matmul(const int8_t* codes, int64_t lda, const float* sca
   a.kbytes = (int)k;
   a.zp = w_zp, a.sums = sums;
   a.bias = bias, a.bias_type = bias_dtype, a.y = y, a.ldy = ldy, a.out_type = out_dtype;
-  a.flags = device_flags();
+  a.flags = status_word();
   if (!a.flags) return fail(IC_ERR_CUDA, "device status word unavailable");
   const Operand x{codes, m, lda, nullptr, scales, 0};
   const Operand w{w_codes, n, ldw, nullptr, w_scales_f16, 1};

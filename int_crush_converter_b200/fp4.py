@@ -36,7 +36,8 @@ class FP4Tensor:
     input's, padded with zeros to a multiple of 32 (and of the rotation size).
     ``scales``: the block-scale bytes, uint8 [ceil(rows/128), ceil(blocks/4), 32, 4, 4]:
     row r, block b at [r//128, b//4, r%32, r%128//32, b%4] (the order in which the
-    product reads them; :meth:`block_scales` gives them row by row).
+    product reads them; :meth:`block_scales` gives them row by row).  The bytes of
+    rows and blocks beyond the matrix are zero.
     ``row_scale``: fp32 [rows] (nvfp4), else None.
     ``lead``: the leading dimensions of the tensor that was quantized (default [rows]).
     """
@@ -64,6 +65,22 @@ class FP4Tensor:
     def to(self, device) -> "FP4Tensor":
         move = lambda t: None if t is None else t.to(device)  # noqa: E731
         return dataclasses.replace(self, packed=move(self.packed), scales=move(self.scales), row_scale=move(self.row_scale))
+
+    @classmethod
+    def from_block_scales(cls, packed: torch.Tensor, block_scales: torch.Tensor, row_scale: torch.Tensor | None = None,
+                          fmt: str = "mxfp4", **kw) -> "FP4Tensor":
+        """From block-scale bytes kept row by row, uint8 [rows, blocks] (E8M0 or E4M3), as :meth:`block_scales` gives them."""
+        if fmt not in FORMATS:
+            raise ValueError(f"fmt must be one of {sorted(FORMATS)}, got {fmt!r}")
+        rows, blocks = packed.shape[0], 2 * packed.shape[1] // BLOCK[fmt]
+        if tuple(block_scales.shape) != (rows, blocks) or block_scales.element_size() != 1:
+            raise ValueError(f"block_scales must be bytes [{rows}, {blocks}], got {block_scales.dtype} {tuple(block_scales.shape)}")
+        a, b = -(-rows // 128), -(-blocks // 4)
+        t = torch.zeros(a * 128, b * 4, dtype=torch.uint8, device=packed.device)
+        t[:rows, :blocks] = block_scales.contiguous().view(torch.uint8)
+        q = cls(packed.contiguous(), t.view(a, 4, 32, b, 4).permute(0, 3, 2, 1, 4).contiguous(), row_scale, fmt, **kw)
+        q.check("from_block_scales")
+        return q
 
     def block_scales(self) -> torch.Tensor:
         """The block-scale bytes as uint8 [rows, blocks]."""

@@ -531,13 +531,74 @@ def test_offsets_beyond_32_bits():
 
 
 def tail(q, n):
-    """The last n rows of q as a tensor of their own (scale tiles rearranged in torch)."""
-    byte = q.block_scales()[-n:]
-    kt = q.scales.shape[1]
-    t = torch.zeros(128, kt * 4, dtype=torch.uint8, device=byte.device)
-    t[:n, :byte.shape[1]] = byte
-    t = t.view(1, 4, 32, kt, 4).permute(0, 3, 2, 1, 4).contiguous()
-    return B.FP4Tensor(q.packed[-n:].contiguous(), t, None if q.row_scale is None else q.row_scale[-n:].contiguous(), q.fmt)
+    """The last n rows of q as a tensor of their own."""
+    return B.FP4Tensor.from_block_scales(q.packed[-n:], q.block_scales()[-n:],
+                                         None if q.row_scale is None else q.row_scale[-n:].contiguous(), q.fmt)
+
+
+FIRST_IN_CAPTURE = """
+import torch
+import int_crush_converter_b200 as B
+x = torch.randn(5, 256, device="cuda")
+w = torch.randn(256, device="cuda")
+codes = torch.randint(-9, 10, (48, 256), device="cuda").to(torch.int8)
+scales = torch.ones(48, 1, device="cuda").half()
+torch.cuda.synchronize()
+def f():
+    q, _ = B.rmsnorm_quantize(x, w)
+    p = B.quantize_fp4(x, "nvfp4", rot_size=64)
+    return B.matmul_int8(q, codes, scales), B.matmul_fp4(p, p), B.dequantize_fp4(p), B.dequantize_int8(q)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = f()
+g.replay()
+torch.cuda.synchronize()
+for a, b in zip(out, f()):
+    assert torch.equal(a, b)
+print("captured")
+"""
+
+
+def test_first_calls_may_be_captured():
+    """A process whose first calls of the library are part of a stream capture."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("m,k", [(1, 32), (128, 128), (129, 512), (300, 1000)])
+def test_block_scales_round_trip(fmt, m, k):
+    q = B.quantize_fp4(rows(m, m, k), fmt)
+    p = B.FP4Tensor.from_block_scales(q.packed, q.block_scales(), q.row_scale, fmt)
+    assert torch.equal(p.scales, q.scales) and torch.equal(B.dequantize_fp4(p), B.dequantize_fp4(q))
+
+
+@pytest.mark.parametrize("kind", ["mxfp4", "nvfp4", "int8"])
+def test_products_on_two_streams_at_once(kind):
+    """Large and small products overlapping on two streams give what they give alone."""
+    big, small, w = rows(1, 2600, 1024), rows(2, 3, 1024), rows(3, 2400, 1024)
+    if kind == "int8":
+        c = torch.randint(-99, 100, (2400, 1024), device="cuda", generator=gen(5)).to(torch.int8)
+        s = torch.ones(2400, 1, device="cuda").half()
+        one = torch.ones(1024, device="cuda")
+        qb, qs = B.rmsnorm_quantize(big, one)[0], B.rmsnorm_quantize(small, one)[0]
+        f = lambda q: B.matmul_int8(q, c, s)  # noqa: E731
+    else:
+        qw, qb, qs = (B.quantize_fp4(t, kind) for t in (w, big, small))
+        f = lambda q: B.matmul_fp4(q, qw)  # noqa: E731
+    want = f(qb), f(qs)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append((i % 3 == 0, f(qb) if i % 3 == 0 else f(qs)))
+    torch.cuda.synchronize()
+    for large, y in got:
+        assert torch.equal(y, want[0] if large else want[1])
 
 
 def test_no_timeouts_were_recorded():

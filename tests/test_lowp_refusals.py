@@ -125,3 +125,13 @@ def test_c_entry_points_refuse_before_any_launch():
     for bad in (dict(fmt=5), dict(wt=4), dict(eps=-1.0), dict(w=None), dict(r=p, ldr=64), dict(r=p, ldr=64, ro=p), dict(ldq=48),
                 dict(ldq=72), dict(g=None), dict(rot=2), dict(kp=65), dict(fmt=1, ldq=32, s=None)):
         assert rn(**bad) == inv, bad
+
+
+def test_block_scales_of_another_shape():
+    p = torch.zeros(4, 32, dtype=torch.uint8)
+    for bad, fmt in ((torch.zeros(4, 3, dtype=torch.uint8), "mxfp4"), (torch.zeros(4, 2, dtype=torch.int16), "mxfp4"),
+                     (torch.zeros(4, 2, dtype=torch.uint8), "nvfp4"), (torch.zeros(4, 2, dtype=torch.uint8), "fp4")):
+        with pytest.raises(ValueError):
+            B.FP4Tensor.from_block_scales(p, bad, None, fmt)
+    q = B.FP4Tensor.from_block_scales(p, torch.arange(8, dtype=torch.uint8).view(4, 2))
+    assert torch.equal(q.block_scales(), torch.arange(8, dtype=torch.uint8).view(4, 2)) and int(q.scales.sum()) == 28
