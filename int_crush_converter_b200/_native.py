@@ -152,6 +152,24 @@ class _Checked:
         return getattr(self.__dict__["_lib"], name)
 
 
+_fast = None
+
+
+def binding():
+    """The native binding of the low-precision operators (``csrc/binding.cpp``): each of its functions
+    does an operator's checks, allocations and call, or returns None for the caller to go the long way."""
+    global _fast
+    if _fast is None:
+        load()
+        try:
+            from . import _binding
+        except ImportError as e:
+            raise ImportError(f"{e}: build the binding with `make -C int_crush_converter_b200/csrc`, with the torch "
+                              "that runs it") from e
+        _fast = _binding
+    return _fast
+
+
 def last_error() -> str:
     return load().ic_last_error().decode(errors="replace")
 

@@ -157,6 +157,10 @@ def quantize_fp4(x: torch.Tensor, fmt: str = "mxfp4", rot_size: int = 0,
     max|x|/2688, so that a row does not depend on its neighbours.  A value that is
     not finite marks its mxfp4 block or its nvfp4 row as NaN.
     """
+    if row_scale is None and fmt in FORMATS:
+        parts = nat.binding().fp4_quantize(x, FORMATS[fmt], rot_size)
+        if parts is not None:
+            return FP4Tensor(*parts, fmt, x.shape[-1], rot_size, x.shape[:-1])
     if fmt not in FORMATS:
         raise ValueError(f"fmt must be one of {sorted(FORMATS)}, got {fmt!r}")
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -191,6 +195,9 @@ def quantize_fp4(x: torch.Tensor, fmt: str = "mxfp4", rot_size: int = 0,
 
 def dequantize_fp4(q: FP4Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values of ``q``, [lead..., columns] (padding included), in fp32/fp16/bf16."""
+    out = nat.binding().fp4_dequantize(q.packed, q.scales, q.row_scale, FORMATS.get(q.fmt, 0), dtype)
+    if out is not None:
+        return out if q.lead is None or len(q.lead) == 1 else out.reshape(*q.lead, out.shape[1])
     q.check("dequantize_fp4")
     if dtype not in _DT:
         raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
@@ -224,6 +231,11 @@ def matmul_fp4(a: FP4Tensor, b: FP4Tensor, bias: torch.Tensor | None = None,
     fp32 and rounded once to ``out_dtype`` (fp32/fp16/bf16).  ``b``'s rows are the
     output's columns.
     """
+    if a.fmt == b.fmt and a.rot_size == b.rot_size and (a.in_features == b.in_features or a.in_features is None or b.in_features is None):
+        y = nat.binding().fp4_matmul(a.packed, a.scales, a.row_scale, b.packed, b.scales, b.row_scale, FORMATS.get(a.fmt, 0), bias,
+                                     out_dtype)
+        if y is not None:
+            return y if a.lead is None or len(a.lead) == 1 else y.reshape(*a.lead, y.shape[1])
     a.check("matmul_fp4")
     b.check("matmul_fp4")
     pa, pb = a.packed, b.packed

@@ -90,6 +90,9 @@ def pitched(codes: torch.Tensor, dev: torch.device) -> tuple[torch.Tensor, int]:
 
 def dequantize_int8(q: Int8Rows, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values of ``q``, [lead..., columns], in fp32/fp16/bf16."""
+    out = nat.binding().int8_dequantize(q.codes, q.scales, dtype)
+    if out is not None:
+        return out if q.lead is None or len(q.lead) == 1 else out.reshape(*q.lead, out.shape[1])
     q.check("dequantize_int8")
     if dtype not in _DT:
         raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
@@ -121,6 +124,9 @@ def matmul_int8(a: Int8Rows, w_codes: torch.Tensor, w_scales: torch.Tensor,
     rows are not 16-byte aligned are copied on every call: keep them at such a
     pitch.
     """
+    y = nat.binding().int8_matmul(a.codes, a.scales, a.sums, w_codes, w_scales, w_zero_points, bias, out_dtype)
+    if y is not None:
+        return y if a.lead is None or len(a.lead) == 1 else y.reshape(*a.lead, y.shape[1])
     a.check("matmul_int8")
     if w_codes.dim() != 2 or w_codes.dtype != torch.int8:
         raise ValueError("matmul_int8: w_codes must be int8 [out, columns]")

@@ -27,6 +27,12 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     """
     if fmt not in _FORMATS:
         raise ValueError(f"fmt must be one of {sorted(_FORMATS)}, got {fmt!r}")
+    parts = nat.binding().rmsnorm_quantize(x, weight, residual, eps, _FORMATS[fmt], rot_size)
+    if parts is not None:
+        a, b, c, h = parts
+        if fmt == "int8":
+            return Int8Rows(a, b, c, x.shape[-1], rot_size, x.shape[:-1]), h
+        return FP4Tensor(a, b, c, fmt, x.shape[-1], rot_size, x.shape[:-1]), h
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("rmsnorm_quantize needs at least one column")
     if x.dtype not in _DT or weight.dtype not in _DT:

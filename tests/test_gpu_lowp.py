@@ -601,6 +601,37 @@ def test_products_on_two_streams_at_once(kind):
         assert torch.equal(y, want[0] if large else want[1])
 
 
+class NoBinding:
+    """Every function of the native binding declines, as for arguments out of the ordinary."""
+
+    def __getattr__(self, name):
+        return lambda *a: None
+
+
+@pytest.mark.parametrize("fmt", ["int8", "mxfp4", "nvfp4"])
+def test_long_way_gives_the_same(fmt, monkeypatch):
+    """With and without the native binding: the same tensors, shapes and types."""
+    x, r = rows(1, 12, 300, torch.bfloat16).reshape(3, 4, 300), rows(2, 12, 300, torch.bfloat16).reshape(3, 4, 300)
+    w, bias = torch.rand(300, device="cuda", generator=gen(3)), torch.rand(70, device="cuda", generator=gen(4))
+    lin = rows(5, 70, 300)
+
+    def layer():
+        q, h = B.rmsnorm_quantize(x, w, residual=r, fmt=fmt, rot_size=32)
+        if fmt == "int8":
+            d = B.rtn_quantize_fused(lin, 32, int_bits=8, asymmetric=True)
+            return [q.codes, q.scales, q.sums, h, B.dequantize_int8(q, torch.float16),
+                    B.matmul_int8(q, d["codes"], d["scales"], d["zero_points"], bias=bias, out_dtype=torch.float32)]
+        p = B.quantize_fp4(lin, fmt, rot_size=32)
+        return [q.packed, q.scales, p.packed, p.scales, h, B.dequantize_fp4(q, torch.float16),
+                B.matmul_fp4(q, p, bias=bias, out_dtype=torch.float32)] + ([] if fmt == "mxfp4" else [q.row_scale, p.row_scale])
+
+    short = layer()
+    monkeypatch.setattr(nat, "_fast", NoBinding())
+    long = layer()
+    assert [(t.shape, t.dtype, t.stride()) for t in short] == [(t.shape, t.dtype, t.stride()) for t in long]
+    assert all(torch.equal(a, b) for a, b in zip(short, long))
+
+
 def test_no_timeouts_were_recorded():
     import ctypes
     f = ctypes.c_uint()
