@@ -17,6 +17,12 @@
 // With few tiles a cluster of S CTAs splits K; each leaves its partial tile in
 // its own shared memory and the cluster adds them in rank order, so the result
 // does not depend on timing.  All waits are bounded (see common.cuh).
+//
+// Measured on B200 (cuBLAS bf16 1700 TFLOP/s, copy 6.56 TB/s): one row x 12288 x
+// 4096 mxfp4 8.9 us with the weights in HBM, 7.5 us from L2 (25 MB: 4.1 us; a
+// launch and its ends alone take 4.2 us); 512 x 4096 x 4096 mxfp4 9.7 us, 300 x
+// 4096 x 16384 nvfp4 20 us (bound by what L2 delivers to narrow tiles); large
+// products run on CTA pairs, below.
 #include <cstdlib>
 
 #include "internal.h"
@@ -575,6 +581,13 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
 // 4608 x 4096 x 16384 nvfp4).  Eight epilogue warps move an accumulator to
 // registers at once and release it; scaling, conversion and stores run under
 // the next products.
+//
+// Measured on B200: 4608 x 16384 x 4096 nvfp4 139 us (4.4 PFLOP/s), 4608 x 4096 x
+// 16384 nvfp4 117 us (5.3), 4608 x 12288 x 4096 int8 150 us (3.1 POP/s), 4608 x
+// 4096 x 16384 int8 200 us (3.1).  Counted in clocks the INT8 main loop runs at
+// 530 a stage of 512 (under the power cap, at 1.5 GHz); the 4-bit ones at 620,
+// because 38 KB a stage is more than five stages in flight bring at L2's latency,
+// and lose 3000 clocks between tiles to the single accumulator.
 //   full[s]  leader only: the bytes of both CTAs' loads
 //   empty[s] in each CTA: the commit of the products that read the stage
 //   accf[b]  in each CTA: the commit of a tile's last product into accumulator b
