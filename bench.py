@@ -531,7 +531,8 @@ def run_device(args, rank: int, world: int) -> None:
                           "frac": round(n_flop / (world * peak_s * 1e12) * 1e3 / ms_step, 4),
                           "note": "whole step's algorithmic flop over N x the sustained 3xTF32 peak "
                                   "(bf16_tflops_sustained / 2 / 3), of measured"},
-        "cpu_baseline": (cpu["cpu_baseline"] if cpu else {"value": None, "unavailable": "reference not installed"}),
+        # the child's line has no baseline where the reference is not installed
+        "cpu_baseline": (cpu or {}).get("cpu_baseline", {"value": None, "unavailable": "reference not installed"}),
         "clocks": clk.summary(),
     }
     print(json.dumps(line), flush=True)
