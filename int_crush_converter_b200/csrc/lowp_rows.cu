@@ -55,6 +55,7 @@ struct RowArgs {
   float* row_scale;
   int32_t* sums;
   int tpr;         // threads per row
+  int tshift, tmask;  // row within the CTA = thread >> tshift, thread within the row = thread & tmask
   int64_t groups;  // row groups, blockDim.x / tpr rows each
 };
 
@@ -175,14 +176,14 @@ __device__ __forceinline__ uint32_t int8x4(float a, float b, float c, float d) {
   return w;
 }
 
-// reductions over the TPR threads of a row (TPR a multiple of 32); `buf` holds
-// one value per warp of the CTA
+// reductions over the TPR threads of a row (TPR a multiple of 32, and a power of
+// two where a CTA has several rows); `buf` holds one value per warp of the CTA
 template <typename V, typename F>
-__device__ __forceinline__ V row_reduce(V v, int tpr, V* buf, F op) {
+__device__ __forceinline__ V row_reduce(V v, int tpr, int tmask, V* buf, F op) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
   if (tpr == 32) return v;
-  const int w = threadIdx.x >> 5, nw = tpr >> 5, w0 = w & ~(nw - 1);
+  const int w = threadIdx.x >> 5, nw = tpr >> 5, w0 = w & ~(tmask >> 5);
   __syncthreads();  // buf may still be read from the last reduction
   if ((threadIdx.x & 31) == 0) buf[w] = v;
   __syncthreads();
@@ -476,7 +477,7 @@ __global__ void __launch_bounds__(NP == 2 ? 512 : 256) rows_kernel(const RowArgs
   __shared__ double buf[32];
   extern __shared__ __align__(16) unsigned char teams[];  // T256: TEAM_BYTES for every 16 threads
   unsigned char* team = teams + (threadIdx.x >> 4) * TEAM_BYTES;
-  const int tpr = a.tpr, t = threadIdx.x & (tpr - 1), rpc = blockDim.x / tpr;
+  const int tpr = a.tpr, t = threadIdx.x & a.tmask, rpc = blockDim.x / tpr;
   const int64_t nch = cdiv(a.kp, 16);
   const int n = NP ? NP : (int)cdiv(nch, 2 * tpr);
   constexpr bool ROW = FMT != IC_MXFP4;  // the codes need the row's largest magnitude
@@ -484,7 +485,7 @@ __global__ void __launch_bounds__(NP == 2 ? 512 : 256) rows_kernel(const RowArgs
   auto ca = [&](int i) { return (int64_t)(2 * i) * tpr + t; };
   auto cb = [&](int i) { return (int64_t)(2 * i + 1) * tpr + t; };
   RawPair<T, NORM> raw[R];
-  int64_t row = (int64_t)blockIdx.x * rpc + threadIdx.x / tpr;
+  int64_t row = (int64_t)blockIdx.x * rpc + (threadIdx.x >> a.tshift);
   if (NP) {
 #pragma unroll
     for (int i = 0; i < R; ++i) raw[i].load(a, row, ca(i), cb(i));
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(NP == 2 ? 512 : 256) rows_kernel(const RowArgs
           ss = fma(y, y, ss);
         }
       }
-      ss = row_reduce(ss, tpr, buf, [](double p, double q) { return p + q; });
+      ss = row_reduce(ss, tpr, a.tmask, buf, [](double p, double q) { return p + q; });
       // squares of fp32 values cannot overflow here: an infinite sum is an infinite input, which marks the whole row
       rstd = isfinite(ss) ? (float)(1.0 / sqrt(ss / (double)a.K + (double)a.eps)) : __int_as_float(0x7fc00000);
     }
@@ -537,7 +538,7 @@ __global__ void __launch_bounds__(NP == 2 ? 512 : 256) rows_kernel(const RowArgs
       float s;
       if (!a.row_scale_in) {
         m = __reduce_max_sync(0xffffffffu, m);
-        m = row_reduce(m, tpr, reinterpret_cast<unsigned*>(buf), [](unsigned p, unsigned q) { return max(p, q); });
+        m = row_reduce(m, tpr, a.tmask, reinterpret_cast<unsigned*>(buf), [](unsigned p, unsigned q) { return max(p, q); });
       }
       if (FMT == IC_INT8) {
         rs.bad = m >= INF_BITS;
@@ -567,7 +568,7 @@ __global__ void __launch_bounds__(NP == 2 ? 512 : 256) rows_kernel(const RowArgs
       sum += emit_pair<FMT>(a, row, ca(i), cb(i), nch, v[k], ma[k], mb[k], rs);
     }
     if (FMT == IC_INT8 && a.sums) {
-      sum = row_reduce(sum, tpr, reinterpret_cast<int*>(buf), [](int p, int q) { return p + q; });
+      sum = row_reduce(sum, tpr, a.tmask, reinterpret_cast<int*>(buf), [](int p, int q) { return p + q; });
       if (t == 0 && row < a.M) a.sums[row] = sum;
     }
   }
@@ -577,15 +578,15 @@ template <typename T, int FMT, bool NORM, int NP, bool T256>
 int launch_np(const RowArgs& a, int threads, cudaStream_t st) {
   const auto kernel = rows_kernel<T, FMT, NORM, NP, T256>;
   const int smem = T256 ? threads / 16 * TEAM_BYTES : 0;
-  // CTAs that the device holds at once, by device and block size (128, 256 or 512 threads)
-  static std::atomic<int> resident[64][3];
+  // CTAs that the device holds at once, by device and warps of a block
+  static std::atomic<int> resident[64][17];
   int dev = 0;
   IC_CUDA(cudaGetDevice(&dev));
-  std::atomic<int>& r = resident[dev & 63][threads == 128 ? 0 : threads == 256 ? 1 : 2];
+  std::atomic<int>& r = resident[dev & 63][threads / 32];
   int ctas = r.load();
   if (!ctas) {
     int sms = 0;
-    if (smem > 48 << 10) IC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (T256) IC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 32 * TEAM_BYTES));
     IC_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, threads, smem));
     IC_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
     ctas = std::max(1, ctas) * sms;
@@ -600,16 +601,20 @@ int launch_np(const RowArgs& a, int threads, cudaStream_t st) {
 template <typename T, int FMT, bool NORM>
 int launch_rows(RowArgs a, cudaStream_t st) {
   const int64_t pairs = cdiv(cdiv(a.kp, 16), 2);
-  // one pair of chunks per thread up to 256 threads, then two, then 512 threads
-  int tpr = 32;
-  while (tpr < 256 && tpr < pairs) tpr *= 2;
-  int np = (int)cdiv(pairs, tpr);
-  if (np > 2 && pairs <= 1024) {
-    tpr = 512;
-    np = 2;
+  // short rows: a power of two of threads, several rows to a CTA; then one row to a CTA with as many
+  // warps as one pair of chunks per thread takes (two pairs beyond 256 threads), up to 512 threads
+  int tpr = 32, np = 1;
+  if (pairs <= 128) {
+    while (tpr < pairs) tpr *= 2;
+  } else {
+    np = pairs <= 256 ? 1 : 2;
+    tpr = (int)std::min<int64_t>(cdiv(cdiv(pairs, np), 32) * 32, 512);
+    if ((int64_t)np * tpr < pairs) np = 0, tpr = 256;  // read again for each reduction
   }
   a.tpr = tpr;
   const int threads = std::max(tpr, 128);
+  a.tshift = threads == tpr ? 10 : ilog2(tpr);
+  a.tmask = (1 << a.tshift) - 1;
   // the 4-bit formats' scale tiles hold 128 rows: the grid covers the padding rows too
   const int64_t rows = FMT == IC_INT8 ? a.M : cdiv(a.M, 128) * 128;
   a.groups = cdiv(rows, threads / tpr);
