@@ -52,7 +52,7 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     lead = x.shape[:-1]
     x2 = as_rows(x, dev)
     r2 = None if residual is None else as_rows(residual, dev)
-    w = weight if weight.is_cuda and weight.is_contiguous() else weight.to(dev).reshape(-1).contiguous()
+    w = weight.to(dev).reshape(-1).contiguous()
     rows, kp = x2.shape[0], padded_columns(k, fmt, rot_size)
     h = None if residual is None else torch.empty(rows, k, dtype=x.dtype, device=dev)
     if fmt == "int8":
