@@ -302,7 +302,10 @@ __device__ __forceinline__ void store_fp4(const RowArgs& a, int64_t row, int64_t
   const int lane = threadIdx.x & 31;
   const uint32_t keep = bad ? 0u : 0xffffffffu;
   const uint2 codes = make_uint2(e2m1x8(y) & keep, e2m1x8(y + 8) & keep);
-  if (row < a.M && c < nch) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.q) + row * a.ldq + c * 8) = codes;
+  const bool in = row < a.M && c < nch;
+  if (in) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.q) + row * a.ldq + c * 8) = codes;
+  // beyond the matrix the norm's 0 times its factor is NaN where that is not finite (a bad row, eps = 0): the bytes there are zero
+  byte = in ? byte : 0u;
   uint32_t word;
   int64_t kt;
   bool first;
