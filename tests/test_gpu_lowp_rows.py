@@ -18,11 +18,81 @@ def rows(seed, m, k, dtype=torch.float32):
     return (torch.randn(m, k, device="cuda", generator=g) * torch.exp(torch.randn(k, device="cuda", generator=g))).to(dtype)
 
 
+def parts(q):
+    """Every tensor of quantized rows, one row of each per row."""
+    if isinstance(q, B.Int8Rows):
+        return [q.codes, q.scales, q.sums]
+    return [q.packed, q.block_scales()] + ([] if q.row_scale is None else [q.row_scale])
+
+
+def same_as_in_batches(f, m, step):
+    """f(first, last) -> tensors of these rows: all rows at once give what `step` rows at a time give."""
+    whole = f(0, m)
+    for i in range(0, m, step):
+        j = min(i + step, m)
+        for a, b in zip(whole, f(i, j)):
+            assert torch.equal(a[i:j], b), (i, j)
+
+
 def beyond(q):
     """The scale bytes beyond the rows and blocks of the matrix."""
     t = q.scales.permute(0, 3, 2, 1, 4).reshape(q.scales.shape[0] * 128, -1).cpu().numpy().copy()
     t[:q.rows, :q.columns // P.BLOCK[q.fmt]] = 0
     return t
+
+
+# More groups of rows than the device holds CTAs, the last one ragged: up to 8192 columns a pair of chunks
+# per thread, up to 32768 two.  60 rows fill at most 128 groups, fewer than the 148 SMs.
+LARGE = [(20001, 96, 32), (5001, 4096, 256), (3001, 5000, 0), (2001, 8192, 64), (1001, 9000, 128), (801, 16384, 256),
+         (601, 32768, 256), (601, 32768, 0)]
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("m,k,rot", LARGE)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quantize_many_groups(fmt, m, k, rot, dtype):
+    x = rows(m, m, k, dtype)
+    same_as_in_batches(lambda i, j: parts(B.quantize_fp4(x[i:j], fmt, rot_size=rot)), m, 60 if k > 512 else 1000)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "mxfp4", "nvfp4"])
+@pytest.mark.parametrize("m,k,rot", LARGE)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rmsnorm_many_groups(fmt, m, k, rot, dtype):
+    x, r = rows(m, m, k, dtype), rows(m + 1, m, k, dtype)
+    w = 1 + 0.1 * rows(3, 1, k)[0].clamp(-3, 3)
+
+    def f(i, j):
+        q, h = B.rmsnorm_quantize(x[i:j], w, residual=r[i:j], fmt=fmt, rot_size=rot)
+        return parts(q) + [h]
+    same_as_in_batches(f, m, 60 if k > 512 else 1000)
+
+
+@pytest.mark.parametrize("m,k,rot", [(5, 16384, 256), (3, 32768, 256), (4, 10000, 256)])
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_wide_rotated_rows(fmt, m, k, rot):
+    """Two pairs of chunks per thread under a rotation of 256: the rotation's own fp32 output, quantized."""
+    x = rows(k, m, k)
+    q, p = B.quantize_fp4(x, fmt, rot_size=rot), B.quantize_fp4(B.rotate_weights(x, rot), fmt)
+    assert all(torch.equal(a, b) for a, b in zip(parts(q), parts(p)))
+
+
+@pytest.mark.parametrize("rot", [0, 16, 32, 64, 128, 256, 512])
+def test_rmsnorm_int8_rounds_each_step(rot):
+    """The norm's products, the scaled value and the addition of 1/2 are rounded one by one.  Of 13 million
+    codes a few dozen lie where a product merged with the addition would choose the other integer."""
+    x, w = rows(rot + 1, 3000, 4480, torch.bfloat16), 1 + 0.3 * rows(2, 1, 4480)[0].clamp(-3, 3)
+    q, _ = B.rmsnorm_quantize(x, w, eps=1e-5, rot_size=rot)
+    h = x.float()
+    rstd = (1.0 / torch.sqrt((h.double() ** 2).mean(1, keepdim=True) + float(np.float32(1e-5)))).float()
+    z = h * rstd * w
+    if rot:
+        z = B.rotate_weights(z, rot)
+    s = (z.abs().amax(1, keepdim=True) * float(np.float32(1 / 127))).clamp(min=1e-30)
+    assert torch.equal(q.scales, s)
+    y = z * (1.0 / s)
+    want = torch.where(y >= 0, torch.floor(y + 0.5), torch.ceil(y - 0.5)).clamp(-128, 127).to(torch.int8)
+    assert torch.equal(q.codes, want)
 
 
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
