@@ -107,3 +107,24 @@ def test_scale_bytes_beyond_the_matrix(fmt, k):
         assert not beyond(q).any()
         v = P.values(q)
         assert np.isfinite(np.delete(v, [3, 129], 0)).all() and np.isnan(v[[3, 129]]).any(1).all()
+
+
+def test_given_row_scales_far_from_one():
+    """Given scales of any size.  u = 2^-24; above 2^120 the reciprocal 1/(6g) is subnormal, at worst 2^-150 of
+    1/(6 * 2^128) > 2^-131 off, i.e. 2^-19 relative; 1/(scale * g), of at least 1/2^128, at worst 2^-22."""
+    for e in (-117, -100, 0, 100, 120, 123, 126, 127):
+        g = float(np.ldexp(1.0, e))
+        x = rows(e + 200, 50, 96) * (0.02 if e < 120 else 0.0002)
+        x = x.clamp(-1, 1) * 300 * g if e < 120 else x.clamp(-1, 1) * 3e38  # within 448 * 6 g and fp32
+        x[:, 32:48] = 0
+        q = B.quantize_fp4(x, "nvfp4", row_scale=g)
+        z = x.double().cpu().numpy()
+        P.check_fp4(q, z, np.abs(z) * (2.0 ** -18 if e >= 120 else 0), given=True)
+        assert not q.packed[:, 16:24].any() and not q.block_scales()[:, 2].any()
+    for g in (2.0 ** -149, 1e-40, 1e-37, 2.0 ** -118):
+        x = torch.zeros(2, 64, device="cuda")
+        x[:, 3], x[:, 5] = 1.0, -1.0  # far above 448 * 6 g: they saturate; zeros stay zero
+        q = B.quantize_fp4(x, "nvfp4", row_scale=g)
+        v, s, h = P.decode(q)
+        assert np.all(s[:, 0] == 448) and not s[:, 1:].any() and np.all(h == float(np.float32(g)))
+        assert np.all(v[:, [3, 5]] == [6, -6]) and np.count_nonzero(v) == 4
