@@ -56,6 +56,12 @@ unsigned long long ic_inverse_graph_count(void);
  * ic_device_status) and returns, leaving the context usable.  Asynchronous
  * on `stream`. */
 int ic_selftest_bounded_wait(unsigned long long limit_ns, void* stream);
+/* Failure-path self-test of the low-precision products (no reference
+ * counterpart): the calling thread's next ic_fp4_matmul or ic_int8_matmul loads
+ * at most `stages` 128-byte stages of K per CTA and its waits give up after
+ * `limit_ns` (0.1 ms .. 2 s).  What stays without its sum becomes NaN in y, and
+ * DEV_TIMEOUT is set. */
+int ic_selftest_matmul_stall(int stages, unsigned long long limit_ns);
 /* Reads and clears the device status word (bit0 timeout, bit1 not-PD,
  * bit2 INT4 range).  Synchronises `stream`. */
 int ic_device_status(unsigned* flags_out, void* stream);
@@ -396,7 +402,9 @@ int ic_int8_row_sums(const int8_t* codes, int64_t ldq, int64_t M, int64_t K, int
 
 /* y [m, n] = a b^T + bias of two 4-bit operands of one format and kp (block-scaled
  * tcgen05 products, fp32 accumulation).  bias per column of y (fp32/fp16/bf16) or
- * NULL; y fp32/fp16/bf16, row pitch ldy. */
+ * NULL; y fp32/fp16/bf16, row pitch ldy.  Asynchronous: should a wait on the
+ * device give up (2 s without progress), DEV_TIMEOUT is set and the elements of
+ * y without their sum are NaN; so too in ic_int8_matmul. */
 int ic_fp4_matmul(const uint8_t* a_packed, const uint8_t* a_scales, const float* a_row_scale,
                   const uint8_t* b_packed, const uint8_t* b_scales, const float* b_row_scale, int fmt,
                   int64_t m, int64_t n, int64_t kp, const void* bias, int bias_dtype, int out_dtype,

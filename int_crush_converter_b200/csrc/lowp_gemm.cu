@@ -16,7 +16,8 @@
 //
 // With few tiles a cluster of S CTAs splits K; each leaves its partial tile in
 // its own shared memory and the cluster adds them in rank order, so the result
-// does not depend on timing.  All waits are bounded (see common.cuh).
+// does not depend on timing.  All waits are bounded (see common.cuh); where one
+// gives up, the elements of y that it leaves without their sums are NaN.
 //
 // Measured on B200 (cuBLAS bf16 1700 TFLOP/s, copy 6.56 TB/s): one row x 12288 x
 // 4096 mxfp4 8.9 us with the weights in HBM, 7.5 us from L2 (25 MB: 4.1 us; a
@@ -33,7 +34,7 @@ namespace {
 
 constexpr int BM = 128;
 constexpr int ROW_BYTES = 128;  // K bytes per stage: one 128-byte swizzle row
-constexpr unsigned long long WAIT_LIMIT_NS = 2000000000ull;
+constexpr unsigned WAIT_LIMIT_NS = 2000000000u;
 constexpr int MAX_SPLIT = 8;
 
 struct LowpArgs {
@@ -51,9 +52,11 @@ struct LowpArgs {
   const int32_t* sums; // row sums of the activations
   const void* bias;    // per weight row
   int bias_type;
+  unsigned wait_ns;    // after which a wait gives up
   void* y;
   long long ldy;
   int out_type;
+  int loads;           // stages that each CTA loads at most (the self-test of waits that give up)
   unsigned* flags;
 };
 
@@ -67,8 +70,8 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, unsigned* flags) {
-  return mbar_wait_bounded(bar, parity, flags, WAIT_LIMIT_NS);
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const LowpArgs& a) {
+  return mbar_wait_bounded(bar, parity, a.flags, a.wait_ns);
 }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* tm, int x, int y, uint32_t bar) {
   asm volatile(
@@ -91,8 +94,8 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 // every lane waits; true where all of them saw the phase complete (the warp stays converged either way)
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, unsigned* flags) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, flags));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const LowpArgs& a) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, a));
 }
 // K-major operand in 128-byte swizzled rows: 8-row groups 1024 bytes apart
 __device__ __forceinline__ uint64_t operand_desc(uint32_t saddr) {
@@ -168,9 +171,10 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
 // What the epilogue applies to a 128 x BN tile: one side of it belongs to the
 // activations (factor, sum of codes), the other to the weights (factor, bias,
 // zero-point).
-struct TileFactors {
+struct alignas(16) TileFactors {
   float rowf[128], rowb[128], colf[256], colb[256];
   int rowi[128], coli[256];
+  unsigned bad;  // 0, or where a wait gave up the bits that make any sum NaN
 };
 
 template <int KIND, int BN>
@@ -192,6 +196,8 @@ struct Cfg {
   static constexpr int TMEM_COLS = TMEM_NEED <= 32 ? 32 : TMEM_NEED <= 64 ? 64 : TMEM_NEED <= 128 ? 128 : TMEM_NEED <= 256 ? 256 : 512;
   static constexpr int SMEM = STAGES * STAGE_BYTES + (int)sizeof(TileFactors) + 1024 /*align*/ + 256 /*barriers*/;
   static_assert(TMEM_NEED <= 512 / CTAS, "tensor memory");
+  static_assert(STAGE_BYTES % 1024 == 0 && sizeof(TileFactors) % 16 == 0, "stages in whole swizzle patterns, barriers on 8 bytes");
+  static_assert(8 * (2 * STAGES + 2) + 4 <= 256, "barriers");
   static_assert(SMEM <= 232448 / CTAS, "shared memory");
   static_assert(BM * BN * 4 <= STAGES * STAGE_BYTES, "a partial tile fits in the stages");
   static constexpr uint32_t IDESC =
@@ -239,6 +245,17 @@ __device__ __forceinline__ T to_out(float v) {
   if constexpr (sizeof(T) == 4) return v;
   else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
   else return __float2bfloat16_rn(v);
+}
+// Where a wait gave up the sums are not there: NaN, so that no caller takes what lies in y for a product.
+// `rows` x `cols` elements of y from element `at`, the lanes side by side along its rows.
+__device__ __forceinline__ void store_nan(const LowpArgs& a, long long at, int rows, int cols, int lane) {
+#pragma unroll 1
+  for (int r = 0; r < rows; ++r, at += a.ldy)
+#pragma unroll 1
+    for (int c = lane; c < cols; c += 32) {
+      if (a.out_type == IC_F32) static_cast<uint32_t*>(a.y)[at + c] = 0x7fffffffu;
+      else static_cast<uint16_t*>(a.y)[at + c] = 0x7fffu;  // in both 16-bit types
+    }
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T* to, const T (&e)[V]) {
@@ -308,6 +325,7 @@ __device__ __forceinline__ void add_parts(const LowpArgs& a, const TileFactors& 
   uint32_t peer[S];
 #pragma unroll
   for (int r = 0; r < S; ++r) peer[r] = map_to_rank(smem_u32(part + c0 * BM + lr), r);
+  const uint32_t lane = threadIdx.x & 31, mark = lane < S ? ld_cluster(map_to_rank(smem_u32(&f.bad), lane)) : 0u;
   const float rowf = f.rowf[lr], rowb = f.rowb[lr];
   const int rowi = f.rowi[lr];
   const bool has_bias = a.bias != nullptr;
@@ -318,6 +336,7 @@ __device__ __forceinline__ void add_parts(const LowpArgs& a, const TileFactors& 
     for (int u = 0; u < V; ++u)
 #pragma unroll
       for (int r = 0; r < S; ++r) v[u][r] = ld_cluster(peer[r] + (uint32_t)((g + u) * BM) * 4u);
+    const uint32_t bad = __reduce_or_sync(0xffffffffu, mark);  // the loop is the same for all lanes
     alignas(16) T e[V];
 #pragma unroll
     for (int u = 0; u < V; ++u) {
@@ -329,7 +348,8 @@ __device__ __forceinline__ void add_parts(const LowpArgs& a, const TileFactors& 
         else s = __float_as_uint(__fadd_rn(__uint_as_float(s), __uint_as_float(v[u][r])));
       }
       const float cf = f.colf[c];
-      e[u] = to_out<T>(finish<KIND>(s, rowi * f.coli[c], a.swap ? cf : rowf, a.swap ? rowf : cf, a.swap ? rowb : f.colb[c], has_bias));
+      const float x = finish<KIND>(s, rowi * f.coli[c], a.swap ? cf : rowf, a.swap ? rowf : cf, a.swap ? rowb : f.colb[c], has_bias);
+      e[u] = to_out<T>(__uint_as_float(__float_as_uint(x) | bad));
     }
     if (row >= a.pm) continue;
     const int col = q0 + c0 + g;
@@ -355,7 +375,7 @@ __device__ __forceinline__ void add_parts(const LowpArgs& a, const TileFactors& 
 //  - split K: partial tiles go to shared memory as [column][128 rows], each CTA
 //    of the cluster adds its share of the columns over the CTAs in rank order.
 template <int KIND, int BN, typename T>
-__device__ __forceinline__ void epilogue(const LowpArgs& a, const TileFactors& f, unsigned char* smem, uint32_t tmem,
+__device__ __forceinline__ void epilogue(const LowpArgs& a, TileFactors& f, unsigned char* smem, uint32_t tmem,
                                          uint32_t acc_bar, int p0, int q0, int rank) {
   constexpr int W = BN < 32 ? 16 : 32;  // columns at a time
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3;
@@ -364,8 +384,7 @@ __device__ __forceinline__ void epilogue(const LowpArgs& a, const TileFactors& f
   uint32_t* part = reinterpret_cast<uint32_t*>(smem);
   if (warp >= 4) {
     asm volatile("bar.sync 1, 128;" ::: "memory");  // the factors are written
-    bool ok = warp_wait(acc_bar, 0, a.flags);
-    if (!ok) warp_wait(acc_bar, 0, a.flags);  // products in flight end before their tensor memory is freed
+    const bool ok = warp_wait(acc_bar, 0, a);
     asm volatile("tcgen05.fence::after_thread_sync;");
     const int lr = q * 32 + lane, row = p0 + lr;
     const float rowf = f.rowf[lr], rowb = f.rowb[lr];
@@ -373,8 +392,14 @@ __device__ __forceinline__ void epilogue(const LowpArgs& a, const TileFactors& f
     constexpr int V = 32 / sizeof(T);
     const uintptr_t at_y = reinterpret_cast<uintptr_t>(y) | (uintptr_t)(a.ldy * (long long)sizeof(T));
     const bool vec = !a.swap && (at_y & 15) == 0, whole = (at_y & 31) == 0;
-    const int cols = min(BN, a.qn - q0);
-    for (int c = 0; c < cols; c += W) {
+    const int cols = min(BN, a.qn - q0), rows = min(32, a.pm - p0 - q * 32);
+    if (!ok && a.splits > 1) {
+      f.bad = 0x7fffffffu;
+    } else if (!ok) {
+      if (a.swap) store_nan(a, (long long)q0 * a.ldy + p0 + q * 32, cols, rows, lane);
+      else store_nan(a, (long long)(p0 + q * 32) * a.ldy + q0, rows, cols, lane);
+    }
+    for (int c = 0; ok && c < cols; c += W) {
       uint32_t r[W];
       const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c;
       if constexpr (W == 16) IC_TMEM_LD16(at, r);
@@ -385,7 +410,6 @@ __device__ __forceinline__ void epilogue(const LowpArgs& a, const TileFactors& f
         for (int j = 0; j < W; ++j) part[(c + j) * BM + lr] = r[j];
         continue;
       }
-      if (!ok) continue;
       float v[W];
 #pragma unroll
       for (int j = 0; j < W; ++j) {
@@ -425,7 +449,7 @@ __device__ __forceinline__ void epilogue(const LowpArgs& a, const TileFactors& f
           float part_v[C];
 #pragma unroll
           for (int u = 0; u < C; ++u) part_v[u] = v[g + u];
-          store_rows<T, C>(mine, part_v, min(32, a.pm - p0 - q * 32), min(C, cols - c - g),
+          store_rows<T, C>(mine, part_v, rows, min(C, cols - c - g),
                            y + (long long)(p0 + q * 32) * a.ldy + q0 + c + g, a.ldy, lane);
         }
       }
@@ -451,10 +475,10 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   TileFactors& f = *reinterpret_cast<TileFactors*>(smem + STAGES * C::STAGE_BYTES);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE_BYTES + sizeof(TileFactors));
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 2);
   auto full_bar = [&](int s) { return smem_u32(bars + s); };
   auto empty_bar = [&](int s) { return smem_u32(bars + STAGES + s); };
-  const uint32_t acc_bar = smem_u32(bars + 2 * STAGES);
+  const uint32_t acc_bar = smem_u32(bars + 2 * STAGES), last_bar = smem_u32(bars + 2 * STAGES + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile = blockIdx.x / a.splits, rank = blockIdx.x - tile * a.splits;
@@ -471,6 +495,8 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
       mbar_init(empty_bar(s), 1);
     }
     mbar_init(acc_bar, 1);
+    mbar_init(last_bar, 1);
+    f.bad = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
@@ -486,9 +512,9 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer ----------------
     int issued = 0;
-    for (int i = 0; i < n; ++i) {
+    for (int i = 0; i < min(n, a.loads); ++i) {
       const int s = i % STAGES;
-      if (i >= STAGES && !mbar_wait(empty_bar(s), ((i / STAGES) & 1) ^ 1, a.flags)) break;
+      if (i >= STAGES && !mbar_wait(empty_bar(s), ((i / STAGES) & 1) ^ 1, a)) break;
       const int kt = kt0 + i;
       const uint32_t base = smem_u32(smem + s * C::STAGE_BYTES);
       uint32_t bytes = C::P_BYTES + C::Q_BYTES, sf = 0;
@@ -511,7 +537,8 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
       issued = i + 1;
     }
     // no copy of this CTA is in flight when it leaves (already true unless a wait gave up)
-    for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(full_bar(i % STAGES), (i / STAGES) & 1, a.flags);
+    for (int i = max(0, issued - STAGES); i < issued; ++i)
+      mbar_wait_bounded(full_bar(i % STAGES), (i / STAGES) & 1, a.flags, WAIT_LIMIT_NS);
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     const uint32_t base0 = smem_u32(smem), sf0 = tmem + C::ACC_COLS;
@@ -519,8 +546,10 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
     const uint32_t qcol = C::FP4 ? (uint32_t)((q0 & 127) >> 5) : 0u;  // narrow tiles start inside a 128-row scale tile
     int s = 0, left = a.kbytes - kt0 * ROW_BYTES;
     uint32_t ph = 0;
+    bool ok = true;
     for (int i = 0; i < n; ++i, left -= ROW_BYTES) {
-      if (!warp_wait(full_bar(s), ph, a.flags)) break;
+      ok = warp_wait(full_bar(s), ph, a);
+      if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;");
       const uint32_t at = (uint32_t)(s * C::STAGE_BYTES) >> 4;  // the descriptors' address field counts 16 bytes
       const uint32_t sfp = sf0 + s * C::SF_COLS, sfq = sfp + C::SF_TILES * 4;
@@ -553,6 +582,10 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
         ph ^= 1;
       }
     }
+    // products in flight end before their tensor memory is freed
+    if (!ok && elect_one()) mma_commit(last_bar);
+    __syncwarp();
+    mbar_wait_bounded(ok ? acc_bar : last_bar, 0, a.flags, WAIT_LIMIT_NS);
   }
   __syncwarp();
 
@@ -593,6 +626,7 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
 //   accf[b]  in each CTA: the commit of a tile's last product into accumulator b
 //   acce[b]  leader only: 16 epilogue warps have taken accumulator b
 //   facf/face[b] in each CTA: the tile's factors are loaded / have been read
+//   last     leader only: the commit of the products before a wait that gave up
 // What the epilogue applies to one 128 x 256 part of a tile
 struct Factors {
   float col[256], bias[256], row[128];
@@ -616,6 +650,8 @@ struct PairCfg {
   static constexpr int OUT_BYTES = 8 * 32 * ROW_PITCH;  // per epilogue warp: 32 rows of 64 bytes
   static constexpr int SMEM = STAGES * STAGE_BYTES + OUT_BYTES + 2 * (int)sizeof(Factors) + 1024 + 256;
   static_assert(NACC * BN + STAGES * SF_COLS <= TMEM_COLS, "tensor memory");
+  static_assert(STAGE_BYTES % 1024 == 0 && OUT_BYTES % 16 == 0 && sizeof(Factors) % 16 == 0, "stages in whole swizzle patterns, barriers on 8 bytes");
+  static_assert(8 * (2 * STAGES + 9) + 4 <= 256, "barriers");
   static_assert(SMEM <= 232448, "shared memory");
   static constexpr uint32_t IDESC =
       KIND == IC_INT8 ? (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(256 >> 4) << 24)
@@ -667,6 +703,9 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(mask)
       : "memory");
+}
+__device__ __forceinline__ void mma_commit_leader(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -757,13 +796,14 @@ __global__ void __launch_bounds__(384, 1)
   unsigned char* out_smem = smem + STAGES * C::STAGE_BYTES;
   Factors* factors = reinterpret_cast<Factors*>(out_smem + C::OUT_BYTES);  // two, by turns
   uint64_t* bars = reinterpret_cast<uint64_t*>(out_smem + C::OUT_BYTES + 2 * sizeof(Factors));
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 8);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 9);
   auto full_bar = [&](int s) { return smem_u32(bars + s); };
   auto empty_bar = [&](int s) { return smem_u32(bars + STAGES + s); };
   auto accf = [&](int b) { return smem_u32(bars + 2 * STAGES + b); };
   auto acce = [&](int b) { return smem_u32(bars + 2 * STAGES + 2 + b); };
   auto facf = [&](int b) { return smem_u32(bars + 2 * STAGES + 4 + b); };
   auto face = [&](int b) { return smem_u32(bars + 2 * STAGES + 6 + b); };
+  const uint32_t last_bar = smem_u32(bars + 2 * STAGES + 8);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -789,6 +829,7 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(facf(b), 32);
       mbar_init(face(b), 8);
     }
+    mbar_init(last_bar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
@@ -811,7 +852,7 @@ __global__ void __launch_bounds__(384, 1)
       place(tile, p0, q0);
       for (int i = 0; i < n; ++i, ++g) {
         const int s = g % STAGES;
-        if (g >= STAGES && !mbar_wait(empty_bar(s), ((g / STAGES) & 1) ^ 1, a.flags)) {
+        if (g >= a.loads || (g >= STAGES && !mbar_wait(empty_bar(s), ((g / STAGES) & 1) ^ 1, a))) {
           ok = false;
           break;
         }
@@ -829,7 +870,8 @@ __global__ void __launch_bounds__(384, 1)
     }
     // no copy is in flight when the pair leaves (already true unless a wait gave up)
     if (leader)
-      for (int i = max(0, g - STAGES); i < g; ++i) mbar_wait(full_bar(i % STAGES), (i / STAGES) & 1, a.flags);
+      for (int i = max(0, g - STAGES); i < g; ++i)
+        mbar_wait_bounded(full_bar(i % STAGES), (i / STAGES) & 1, a.flags, WAIT_LIMIT_NS);
   } else if (warp == 1 && leader) {
     // ---------------- MMA issuer (leader) ----------------
     const uint32_t base0 = smem_u32(smem);
@@ -839,15 +881,14 @@ __global__ void __launch_bounds__(384, 1)
     bool ok = true;
     for (int tile = pair; tile < tiles && ok; tile += pairs, ++t) {
       const int b = t % C::NACC;
-      if (t >= C::NACC && !warp_wait(acce(b), ((t / C::NACC) & 1) ^ 1, a.flags)) break;
+      if (t >= C::NACC) ok = warp_wait(acce(b), ((t / C::NACC) & 1) ^ 1, a);
+      if (!ok) break;
       const uint32_t acc = tmem + b * C::BN;
       asm volatile("tcgen05.fence::after_thread_sync;");
       int left = a.kbytes;
       for (int i = 0; i < n; ++i, left -= ROW_BYTES) {
-        if (!warp_wait(full_bar(s), ph, a.flags)) {
-          ok = false;
-          break;
-        }
+        ok = warp_wait(full_bar(s), ph, a);
+        if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;");
         const uint32_t at = (uint32_t)(s * C::STAGE_BYTES) >> 4;  // the descriptors' address field counts 16 bytes
         const uint32_t sfp = tmem + C::BN + s * C::SF_COLS, sfq = sfp + C::SF_TILES * 4;
@@ -878,6 +919,10 @@ __global__ void __launch_bounds__(384, 1)
         }
       }
     }
+    // products in flight end before their tensor memory is freed
+    if (!ok && elect_one()) mma_commit_leader(last_bar);
+    __syncwarp();
+    mbar_wait_bounded(ok ? accf((t - 1) % C::NACC) : last_bar, ok ? ((t - 1) / C::NACC) & 1 : 0, a.flags, WAIT_LIMIT_NS);
   } else if (warp == 3) {
     // ---------------- factors of the coming tile (both CTAs) ----------------
     int t = 0;
@@ -885,7 +930,7 @@ __global__ void __launch_bounds__(384, 1)
       int p0, q0;
       place(tile, p0, q0);
       Factors& f = factors[t & 1];
-      if (t >= 2 && !warp_wait(face(t & 1), ((t >> 1) & 1) ^ 1, a.flags)) break;
+      if (t >= 2 && !warp_wait(face(t & 1), ((t >> 1) & 1) ^ 1, a)) break;
       const int row0 = p0 + (int)rank * 128;
       float cf[8], cb[8], rf[4];
       load_strided(a.q_row, a.q_half ? IC_F16 : IC_F32, q0 + lane, a.qn, cf);
@@ -920,15 +965,13 @@ __global__ void __launch_bounds__(384, 1)
     // ---------------- epilogue (both CTAs, own rows) ----------------
     const int q = warp & 3, h = (warp - 4) >> 2;
     unsigned char* out = out_smem + (warp - 4) * (32 * ROW_PITCH);
-    int t = 0;
-    for (int tile = pair; tile < tiles; tile += pairs, ++t) {
+    int t = 0, tile = pair;
+    for (; tile < tiles; tile += pairs, ++t) {
       int p0, q0;
       place(tile, p0, q0);
       const int row0 = p0 + (int)rank * 128 + q * 32, col0 = q0 + h * 128;
-      bool ok = warp_wait(facf(t & 1), (t >> 1) & 1, a.flags);
       const int b = t % C::NACC;
-      ok &= warp_wait(accf(b), (t / C::NACC) & 1, a.flags);
-      if (!ok) warp_wait(accf(b), (t / C::NACC) & 1, a.flags);  // products in flight end before their tensor memory is freed
+      if (!warp_wait(facf(t & 1), (t >> 1) & 1, a) || !warp_wait(accf(b), (t / C::NACC) & 1, a)) break;
       asm volatile("tcgen05.fence::after_thread_sync;");
       uint32_t acc[128];
       const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * C::BN + h * 128);
@@ -938,13 +981,18 @@ __global__ void __launch_bounds__(384, 1)
       asm volatile("tcgen05.fence::before_thread_sync;");
       __syncwarp();
       if (lane == 0) remote_arrive(map_to_rank(acce(b), 0));
-      if (!ok) break;
       const Factors& f = factors[t & 1];
       if (a.out_type == IC_BF16) store_block<KIND, __nv_bfloat16>(a, acc, out, f, q * 32, h * 128, row0, col0, lane);
       else if (a.out_type == IC_F16) store_block<KIND, __half>(a, acc, out, f, q * 32, h * 128, row0, col0, lane);
       else store_block<KIND, float>(a, acc, out, f, q * 32, h * 128, row0, col0, lane);
       __syncwarp();
       if (lane == 0) mbar_arrive(face(t & 1));  // every lane has read the factors
+    }
+    for (; tile < tiles; tile += pairs) {  // a wait gave up: nor is a later tile of this warp's computed
+      int p0, q0;
+      place(tile, p0, q0);
+      const int row0 = p0 + (int)rank * 128 + q * 32, col0 = q0 + h * 128;
+      store_nan(a, (long long)row0 * a.ldy + col0, min(32, a.pm - row0), min(128, a.qn - col0), lane);
     }
   }
   __syncwarp();
@@ -1189,8 +1237,31 @@ unsigned* status_word() {
   return r == IC_OK ? device_flags() : nullptr;
 }
 
+// What the next product of this thread is to load, and how long its waits last
+struct Stall {
+  int loads = INT32_MAX;
+  unsigned wait_ns = WAIT_LIMIT_NS;
+};
+thread_local Stall g_stall;
+
+int set_waits(LowpArgs& a) {
+  a.flags = status_word();
+  if (!a.flags) return fail(IC_ERR_CUDA, "device status word unavailable");
+  a.loads = g_stall.loads, a.wait_ns = g_stall.wait_ns;
+  g_stall = Stall{};
+  return IC_OK;
+}
+
 }  // namespace
 }  // namespace ic
+
+extern "C" int ic_selftest_matmul_stall(int stages, unsigned long long limit_ns) {
+  using namespace ic;
+  if (stages < 0 || limit_ns < 100000ull || limit_ns > WAIT_LIMIT_NS)
+    return fail(IC_ERR_INVALID, "selftest: stages must not be negative, the wait limit in [0.1 ms, 2 s]");
+  g_stall = Stall{stages, (unsigned)limit_ns};
+  return IC_OK;
+}
 
 extern "C" int ic_fp4_matmul(const uint8_t* a_packed, const uint8_t* a_scales, const float* a_row_scale,
                              const uint8_t* b_packed, const uint8_t* b_scales, const float* b_row_scale, int fmt,
@@ -1209,8 +1280,7 @@ extern "C" int ic_fp4_matmul(const uint8_t* a_packed, const uint8_t* a_scales, c
   a.kbytes = (int)(kp / 2);
   a.ktiles = (int)fp4_ktiles(fmt, kp);
   a.bias = bias, a.bias_type = bias_dtype, a.y = y, a.ldy = ldy, a.out_type = out_dtype;
-  a.flags = status_word();
-  if (!a.flags) return fail(IC_ERR_CUDA, "device status word unavailable");
+  IC_TRY(set_waits(a));
   const bool nv = fmt == IC_NVFP4;
   const Operand x{a_packed, m, kp / 2, a_scales, nv ? a_row_scale : nullptr, 0};
   const Operand w{b_packed, n, kp / 2, b_scales, nv ? b_row_scale : nullptr, 0};
@@ -1233,8 +1303,7 @@ extern "C" int ic_int8_matmul(const int8_t* codes, int64_t lda, const float* sca
   a.kbytes = (int)k;
   a.zp = w_zp, a.sums = sums;
   a.bias = bias, a.bias_type = bias_dtype, a.y = y, a.ldy = ldy, a.out_type = out_dtype;
-  a.flags = status_word();
-  if (!a.flags) return fail(IC_ERR_CUDA, "device status word unavailable");
+  IC_TRY(set_waits(a));
   const Operand x{codes, m, lda, nullptr, scales, 0};
   const Operand w{w_codes, n, ldw, nullptr, w_scales_f16, 1};
   return matmul<IC_INT8>(x, w, a, (cudaStream_t)stream);
