@@ -174,7 +174,6 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
 struct alignas(16) TileFactors {
   float rowf[128], rowb[128], colf[256], colb[256];
   int rowi[128], coli[256];
-  unsigned bad;  // 0, or where a wait gave up the bits that make any sum NaN
 };
 
 template <int KIND, int BN>
@@ -316,6 +315,9 @@ __device__ __forceinline__ void load_factors(const LowpArgs& a, TileFactors& f, 
   }
 }
 
+// In place of a partial sum where a wait gave up: NaN, or the integer that no sum of int8 products is (k < 2^17)
+constexpr uint32_t NO_SUM = 0x80000000u;
+
 // This CTA's share of a split tile's columns: the S partial sums in rank order, then to y
 template <int KIND, int BN, int S, typename T>
 __device__ __forceinline__ void add_parts(const LowpArgs& a, const TileFactors& f, T* y, const uint32_t* part, int p0, int q0,
@@ -325,7 +327,6 @@ __device__ __forceinline__ void add_parts(const LowpArgs& a, const TileFactors& 
   uint32_t peer[S];
 #pragma unroll
   for (int r = 0; r < S; ++r) peer[r] = map_to_rank(smem_u32(part + c0 * BM + lr), r);
-  const uint32_t lane = threadIdx.x & 31, mark = lane < S ? ld_cluster(map_to_rank(smem_u32(&f.bad), lane)) : 0u;
   const float rowf = f.rowf[lr], rowb = f.rowb[lr];
   const int rowi = f.rowi[lr];
   const bool has_bias = a.bias != nullptr;
@@ -336,20 +337,20 @@ __device__ __forceinline__ void add_parts(const LowpArgs& a, const TileFactors& 
     for (int u = 0; u < V; ++u)
 #pragma unroll
       for (int r = 0; r < S; ++r) v[u][r] = ld_cluster(peer[r] + (uint32_t)((g + u) * BM) * 4u);
-    const uint32_t bad = __reduce_or_sync(0xffffffffu, mark);  // the loop is the same for all lanes
     alignas(16) T e[V];
 #pragma unroll
     for (int u = 0; u < V; ++u) {
       const int c = c0 + g + u;
       uint32_t s = v[u][0];
+      bool bad = KIND == IC_INT8 && s == NO_SUM;
 #pragma unroll
       for (int r = 1; r < S; ++r) {
-        if (KIND == IC_INT8) s += v[u][r];
+        if (KIND == IC_INT8) s += v[u][r], bad |= v[u][r] == NO_SUM;
         else s = __float_as_uint(__fadd_rn(__uint_as_float(s), __uint_as_float(v[u][r])));
       }
       const float cf = f.colf[c];
       const float x = finish<KIND>(s, rowi * f.coli[c], a.swap ? cf : rowf, a.swap ? rowf : cf, a.swap ? rowb : f.colb[c], has_bias);
-      e[u] = to_out<T>(__uint_as_float(__float_as_uint(x) | bad));
+      e[u] = to_out<T>(bad ? __uint_as_float(0x7fffffffu) : x);
     }
     if (row >= a.pm) continue;
     const int col = q0 + c0 + g;
@@ -375,7 +376,7 @@ __device__ __forceinline__ void add_parts(const LowpArgs& a, const TileFactors& 
 //  - split K: partial tiles go to shared memory as [column][128 rows], each CTA
 //    of the cluster adds its share of the columns over the CTAs in rank order.
 template <int KIND, int BN, typename T>
-__device__ __forceinline__ void epilogue(const LowpArgs& a, TileFactors& f, unsigned char* smem, uint32_t tmem,
+__device__ __forceinline__ void epilogue(const LowpArgs& a, const TileFactors& f, unsigned char* smem, uint32_t tmem,
                                          uint32_t acc_bar, int p0, int q0, int rank) {
   constexpr int W = BN < 32 ? 16 : 32;  // columns at a time
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3;
@@ -394,7 +395,7 @@ __device__ __forceinline__ void epilogue(const LowpArgs& a, TileFactors& f, unsi
     const bool vec = !a.swap && (at_y & 15) == 0, whole = (at_y & 31) == 0;
     const int cols = min(BN, a.qn - q0), rows = min(32, a.pm - p0 - q * 32);
     if (!ok && a.splits > 1) {
-      f.bad = 0x7fffffffu;
+      for (int c = 0; c < cols; ++c) part[c * BM + lr] = KIND == IC_INT8 ? NO_SUM : 0x7fffffffu;
     } else if (!ok) {
       if (a.swap) store_nan(a, (long long)q0 * a.ldy + p0 + q * 32, cols, rows, lane);
       else store_nan(a, (long long)(p0 + q * 32) * a.ldy + q0, rows, cols, lane);
@@ -496,7 +497,6 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
     }
     mbar_init(acc_bar, 1);
     mbar_init(last_bar, 1);
-    f.bad = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 2) {
@@ -512,7 +512,8 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer ----------------
     int issued = 0;
-    for (int i = 0; i < min(n, a.loads); ++i) {
+    const int loads = min(n, a.loads);
+    for (int i = 0; i < loads; ++i) {
       const int s = i % STAGES;
       if (i >= STAGES && !mbar_wait(empty_bar(s), ((i / STAGES) & 1) ^ 1, a)) break;
       const int kt = kt0 + i;
