@@ -873,6 +873,9 @@ __global__ void __launch_bounds__(384, 1)
     if (leader)
       for (int i = max(0, g - STAGES); i < g; ++i)
         mbar_wait_bounded(full_bar(i % STAGES), (i / STAGES) & 1, a.flags, WAIT_LIMIT_NS);
+    // nor is a commit of the leader's that signals this CTA's barriers
+    for (int i = max(0, g - STAGES); i < g; ++i)
+      if (!mbar_wait(empty_bar(i % STAGES), (i / STAGES) & 1, a)) break;
   } else if (warp == 1 && leader) {
     // ---------------- MMA issuer (leader) ----------------
     const uint32_t base0 = smem_u32(smem);
