@@ -95,6 +95,16 @@ PyObject* guarded(F&& f) {
     return none();
   }
 }
+// f() without the interpreter's lock: an allocation or a launch may wait for the GPU, and what it waits for may
+// need another Python thread
+template <typename F>
+auto unlocked(F&& f) {
+  struct Unlock {
+    PyThreadState* state = PyEval_SaveThread();
+    ~Unlock() { PyEval_RestoreThread(state); }
+  } unlock;
+  return f();
+}
 bool count(Py_ssize_t n, Py_ssize_t want) {
   if (n == want) return true;
   PyErr_Format(PyExc_TypeError, "%zd arguments expected, got %zd", want, n);
@@ -105,6 +115,7 @@ int64_t block_of(long fmt) { return fmt == IC_MXFP4 ? 32 : 16; }
 
 struct Fp4 {
   Tensor packed, scales, row;
+  Fp4() = default;
   Fp4(int64_t rows, int64_t columns, long fmt, int dev)
       : packed(empty({rows, columns / 2}, at::kByte, dev)),
         scales(empty({(rows + 127) / 128, up(columns, 4 * block_of(fmt)) / (4 * block_of(fmt)), 32, 4, 4}, at::kByte, dev)) {
@@ -144,10 +155,13 @@ PyObject* fp4_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int dev = usable_device();
     if (dev != x.t->get_device()) return none();
     const int64_t kp = up(k, std::max<int64_t>(32, rot));
-    Fp4 q(rows, kp, fmt, dev);
-    if (ic_fp4_quantize(x.ptr(), type_code(x.t->scalar_type()), rows, k, pitch, (int)fmt, (int)rot, kp, nullptr, 0,
-                        q.packed.data_ptr<uint8_t>(), q.scales.data_ptr<uint8_t>(), q.row.defined() ? q.row.data_ptr<float>() : nullptr,
-                        stream_of(dev)) != IC_OK)
+    Fp4 q;
+    if (unlocked([&] {
+          q = Fp4(rows, kp, fmt, dev);
+          return ic_fp4_quantize(x.ptr(), type_code(x.t->scalar_type()), rows, k, pitch, (int)fmt, (int)rot, kp, nullptr, 0,
+                                 q.packed.data_ptr<uint8_t>(), q.scales.data_ptr<uint8_t>(),
+                                 q.row.defined() ? q.row.data_ptr<float>() : nullptr, stream_of(dev));
+        }) != IC_OK)
       return none();
     return Py_BuildValue("(NNN)", wrap(std::move(q.packed)), wrap(std::move(q.scales)), wrap(std::move(q.row)));
   });
@@ -166,9 +180,12 @@ PyObject* fp4_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int dev = usable_device();
     if (dev < 0 || !is_fp4(p, s, g, fmt, dev)) return none();
     const int64_t rows = p.t->size(0), kp = 2 * p.t->size(1);
-    Tensor out = empty({rows, kp}, type, dev);
-    if (ic_fp4_dequantize(p.ptr<uint8_t>(), s.ptr<uint8_t>(), g.ptr<float>(), (int)fmt, rows, kp, code, out.data_ptr(), kp,
-                          stream_of(dev)) != IC_OK)
+    Tensor out;
+    if (unlocked([&] {
+          out = empty({rows, kp}, type, dev);
+          return ic_fp4_dequantize(p.ptr<uint8_t>(), s.ptr<uint8_t>(), g.ptr<float>(), (int)fmt, rows, kp, code, out.data_ptr(), kp,
+                                   stream_of(dev));
+        }) != IC_OK)
       return none();
     return wrap(std::move(out));
   });
@@ -188,10 +205,13 @@ PyObject* fp4_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (dev < 0 || !is_fp4(pa, sa, ga, fmt, dev) || !is_fp4(pb, sb, gb, fmt, dev)) return none();
     const int64_t m = pa.t->size(0), w = pb.t->size(0), kp = 2 * pa.t->size(1);
     if (pa.t->size(1) != pb.t->size(1) || !is_bias(bias, w, dev)) return none();
-    Tensor y = empty({m, w}, type, dev);
-    if (ic_fp4_matmul(pa.ptr<uint8_t>(), sa.ptr<uint8_t>(), ga.ptr<float>(), pb.ptr<uint8_t>(), sb.ptr<uint8_t>(),
-                      gb.ptr<float>(), (int)fmt, m, w, kp, bias.ptr(), bias.t ? type_code(bias.t->scalar_type()) : 0, code,
-                      y.data_ptr(), w, stream_of(dev)) != IC_OK)
+    Tensor y;
+    if (unlocked([&] {
+          y = empty({m, w}, type, dev);
+          return ic_fp4_matmul(pa.ptr<uint8_t>(), sa.ptr<uint8_t>(), ga.ptr<float>(), pb.ptr<uint8_t>(), sb.ptr<uint8_t>(),
+                               gb.ptr<float>(), (int)fmt, m, w, kp, bias.ptr(), bias.t ? type_code(bias.t->scalar_type()) : 0, code,
+                               y.data_ptr(), w, stream_of(dev));
+        }) != IC_OK)
       return none();
     return wrap(std::move(y));
   });
@@ -214,24 +234,31 @@ PyObject* rmsnorm_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (dev != x.t->get_device() || dev != w.t->get_device()) return none();
     if (r.t && (!r.on(dev, x.t->scalar_type()) || r.t->sizes() != x.t->sizes() || !rows_of(*r.t, rrows, rk, rpitch))) return none();
     Tensor h;
-    if (r.t) h = empty(x.t->sizes(), x.t->scalar_type(), dev);
     const int xt = type_code(x.t->scalar_type()), wt = type_code(w.t->scalar_type());
-    void* st = stream_of(dev);
     if (fmt == IC_INT8) {
       const int64_t kp = up(k, std::max<int64_t>(1, rot)), ld = up(kp, 16);
-      Tensor codes = empty({rows, ld}, at::kChar, dev), scales = empty({rows, 1}, at::kFloat, dev), sums = empty({rows}, at::kInt, dev);
-      if (ic_rmsnorm_quantize(x.ptr(), r.ptr(), xt, rows, k, pitch, rpitch, w.ptr(), wt, (float)eps, (int)fmt, (int)rot, kp,
-                              h.defined() ? h.data_ptr() : nullptr, k, codes.data_ptr(), ld, nullptr, scales.data_ptr<float>(),
-                              sums.data_ptr<int32_t>(), st) != IC_OK)
+      Tensor codes, scales, sums;
+      if (unlocked([&] {
+            if (r.t) h = empty(x.t->sizes(), x.t->scalar_type(), dev);
+            codes = empty({rows, ld}, at::kChar, dev), scales = empty({rows, 1}, at::kFloat, dev), sums = empty({rows}, at::kInt, dev);
+            return ic_rmsnorm_quantize(x.ptr(), r.ptr(), xt, rows, k, pitch, rpitch, w.ptr(), wt, (float)eps, (int)fmt, (int)rot, kp,
+                                       h.defined() ? h.data_ptr() : nullptr, k, codes.data_ptr(), ld, nullptr,
+                                       scales.data_ptr<float>(), sums.data_ptr<int32_t>(), stream_of(dev));
+          }) != IC_OK)
         return none();
       if (ld != kp) codes = codes.narrow(1, 0, kp);
       return Py_BuildValue("(NNNN)", wrap(std::move(codes)), wrap(std::move(scales)), wrap(std::move(sums)), wrap(std::move(h)));
     }
     const int64_t kp = up(k, std::max<int64_t>(32, rot));
-    Fp4 q(rows, kp, fmt, dev);
-    if (ic_rmsnorm_quantize(x.ptr(), r.ptr(), xt, rows, k, pitch, rpitch, w.ptr(), wt, (float)eps, (int)fmt, (int)rot, kp,
-                            h.defined() ? h.data_ptr() : nullptr, k, q.packed.data_ptr(), kp / 2, q.scales.data_ptr<uint8_t>(),
-                            q.row.defined() ? q.row.data_ptr<float>() : nullptr, nullptr, st) != IC_OK)
+    Fp4 q;
+    if (unlocked([&] {
+          if (r.t) h = empty(x.t->sizes(), x.t->scalar_type(), dev);
+          q = Fp4(rows, kp, fmt, dev);
+          return ic_rmsnorm_quantize(x.ptr(), r.ptr(), xt, rows, k, pitch, rpitch, w.ptr(), wt, (float)eps, (int)fmt, (int)rot, kp,
+                                     h.defined() ? h.data_ptr() : nullptr, k, q.packed.data_ptr(), kp / 2,
+                                     q.scales.data_ptr<uint8_t>(), q.row.defined() ? q.row.data_ptr<float>() : nullptr, nullptr,
+                                     stream_of(dev));
+        }) != IC_OK)
       return none();
     return Py_BuildValue("(NNNN)", wrap(std::move(q.packed)), wrap(std::move(q.scales)), wrap(std::move(q.row)), wrap(std::move(h)));
   });
@@ -261,8 +288,12 @@ PyObject* int8_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
     int64_t pitch;
     if (dev < 0 || !is_codes(c, dev, false, pitch) || !per_row(s, c.t->size(0), dev, at::kFloat)) return none();
     const int64_t rows = c.t->size(0), k = c.t->size(1);
-    Tensor out = empty({rows, k}, type, dev);
-    if (ic_int8_dequantize(c.ptr<int8_t>(), pitch, s.ptr<float>(), rows, k, code, out.data_ptr(), k, stream_of(dev)) != IC_OK) return none();
+    Tensor out;
+    if (unlocked([&] {
+          out = empty({rows, k}, type, dev);
+          return ic_int8_dequantize(c.ptr<int8_t>(), pitch, s.ptr<float>(), rows, k, code, out.data_ptr(), k, stream_of(dev));
+        }) != IC_OK)
+      return none();
     return wrap(std::move(out));
   });
 }
@@ -284,10 +315,13 @@ PyObject* int8_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return none();
     if (zp.t && (!per_row(zp, nw, dev, at::kChar) || !per_row(sums, m, dev, at::kInt))) return none();
     if (sums.t && !per_row(sums, m, dev, at::kInt)) return none();
-    Tensor y = empty({m, nw}, type, dev);
-    if (ic_int8_matmul(c.ptr<int8_t>(), lda, s.ptr<float>(), sums.ptr<int32_t>(), w.ptr<int8_t>(), ldw,
-                       ws.ptr<uint16_t>(), zp.ptr<int8_t>(), m, nw, k, bias.ptr(), bias.t ? type_code(bias.t->scalar_type()) : 0,
-                       code, y.data_ptr(), nw, stream_of(dev)) != IC_OK)
+    Tensor y;
+    if (unlocked([&] {
+          y = empty({m, nw}, type, dev);
+          return ic_int8_matmul(c.ptr<int8_t>(), lda, s.ptr<float>(), sums.ptr<int32_t>(), w.ptr<int8_t>(), ldw, ws.ptr<uint16_t>(),
+                                zp.ptr<int8_t>(), m, nw, k, bias.ptr(), bias.t ? type_code(bias.t->scalar_type()) : 0, code,
+                                y.data_ptr(), nw, stream_of(dev));
+        }) != IC_OK)
       return none();
     return wrap(std::move(y));
   });
