@@ -8,8 +8,10 @@ missing, or no sm_100 GPU is present, every quantization call raises.
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
 import threading
+import warnings
 
 import torch
 
@@ -156,18 +158,27 @@ class _Checked:
 _fast = None
 
 
+class _NoBinding:
+    """Stands in for the native binding where it was not built: every function declines."""
+
+    def __getattr__(self, name):
+        return lambda *a: None
+
+
 def binding():
     """The native binding of the low-precision operators (``csrc/binding.cpp``): each of its functions
     does an operator's checks, allocations and call, or returns None for the caller to go the long way."""
     global _fast
     if _fast is None:
         load()
+        build = "build the binding with `make -C int_crush_converter_b200/csrc`, with the torch that runs it"
         try:
-            from . import _binding
+            _fast = importlib.import_module("._binding", __package__)
+        except ModuleNotFoundError:
+            warnings.warn(f"_binding.so is missing, calls take about 8 us of host time more: {build}", RuntimeWarning, stacklevel=3)
+            _fast = _NoBinding()
         except ImportError as e:
-            raise ImportError(f"{e}: build the binding with `make -C int_crush_converter_b200/csrc`, with the torch "
-                              "that runs it") from e
-        _fast = _binding
+            raise ImportError(f"{e}: {build}") from e
     return _fast
 
 
