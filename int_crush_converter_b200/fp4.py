@@ -84,8 +84,8 @@ class FP4Tensor:
 
     def block_scales(self) -> torch.Tensor:
         """The block-scale bytes as uint8 [rows, blocks]."""
-        a, b = self.scales.shape[:2]
-        t = self.scales.permute(0, 3, 2, 1, 4).reshape(a * 128, b * 4)
+        a, b = -(-self.rows // 128), _ktiles(self.fmt, self.columns)
+        t = self.scales.reshape(a, b, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(a * 128, b * 4)
         return t[:self.rows, :self.columns // BLOCK[self.fmt]].contiguous()
 
     def check(self, what: str) -> None:

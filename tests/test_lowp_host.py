@@ -71,3 +71,13 @@ def test_a_binding_that_does_not_load_is_an_error(monkeypatch):
     monkeypatch.setattr(importlib, "import_module", load)
     with pytest.raises(ImportError, match="undefined symbol.*make -C"):
         nat.binding()
+
+
+@pytest.mark.parametrize("fmt,blocks", [("mxfp4", 10), ("nvfp4", 20)])
+def test_block_scales_of_flat_scale_bytes(fmt, blocks):
+    """Scale bytes are taken in any shape; row by row they are the same."""
+    want = torch.randint(0, 100, (130, blocks), dtype=torch.uint8)
+    q = B.FP4Tensor.from_block_scales(torch.zeros(130, 160, dtype=torch.uint8), want, None if fmt == "mxfp4" else torch.ones(130), fmt)
+    q.scales = q.scales.reshape(-1)
+    q.check("test")
+    assert torch.equal(q.block_scales(), want)
