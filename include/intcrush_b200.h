@@ -62,6 +62,13 @@ int ic_selftest_bounded_wait(unsigned long long limit_ns, void* stream);
  * `limit_ns` (0.1 ms .. 2 s).  What stays without its sum becomes NaN in y, and
  * DEV_TIMEOUT is set. */
 int ic_selftest_matmul_stall(int stages, unsigned long long limit_ns);
+/* Self-test of the same products (no reference counterpart): the calling
+ * thread's next one is cut into 128-row tiles of `width` columns (16, 32, 64,
+ * 128, 192, 256; 0: CTA pairs on 256 x 256 tiles, splits 1 and swap 0), with the
+ * weights on the 128-row side if `swap`, and K over `splits` CTAs (1, 2, 4, 8, at
+ * most one per 128 bytes).  IC_ERR_INVALID, here or from the product, where there
+ * is no such plan (16 and 32 take no more rows than their width on that side). */
+int ic_selftest_matmul_plan(int width, int swap, int splits);
 /* Reads and clears the device status word (bit0 timeout, bit1 not-PD,
  * bit2 INT4 range).  Synchronises `stream`. */
 int ic_device_status(unsigned* flags_out, void* stream);

@@ -1195,12 +1195,24 @@ Plan plan(int64_t m, int64_t n, int64_t stages, bool aligned) {
   return best;
 }
 
+// The plan of this thread's next product, where the self-test gives one (splits > 0)
+thread_local Plan g_plan{0, false, 0, 0.0};
+
+// a plan that the kernels can run: narrow tiles cover all rows of Q, every split has a stage, pairs know neither
+bool possible(const Plan& b, int64_t qn, int64_t stages) {
+  return b.bn ? b.splits <= stages && (b.bn > 32 || qn <= b.bn) : b.splits == 1 && !b.swap;
+}
+
 // x [m, k] times w [n, k]^T
 template <int KIND>
 int matmul(const Operand& x, const Operand& w, LowpArgs a, cudaStream_t st) {
   const int64_t size = a.out_type == IC_F32 ? 4 : 2;
   const bool aligned = ((reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)(a.ldy * size)) & 15) == 0;
-  const Plan b = plan<KIND>(x.rows, w.rows, cdiv(a.kbytes, ROW_BYTES), aligned);
+  const int64_t stages = cdiv(a.kbytes, ROW_BYTES);
+  Plan b = g_plan;
+  g_plan.splits = 0;
+  if (!b.splits) b = plan<KIND>(x.rows, w.rows, stages, aligned);
+  else if (!possible(b, b.swap ? x.rows : w.rows, stages)) return fail(IC_ERR_INVALID, "selftest: no such plan of this product");
   a.swap = b.swap;
   const Operand &p = b.swap ? w : x, &q = b.swap ? x : w;
   switch (b.bn) {
@@ -1264,6 +1276,15 @@ extern "C" int ic_selftest_matmul_stall(int stages, unsigned long long limit_ns)
   if (stages < 0 || limit_ns < 100000ull || limit_ns > WAIT_LIMIT_NS)
     return fail(IC_ERR_INVALID, "selftest: stages must not be negative, the wait limit in [0.1 ms, 2 s]");
   g_stall = Stall{stages, (unsigned)limit_ns};
+  return IC_OK;
+}
+
+extern "C" int ic_selftest_matmul_plan(int width, int swap, int splits) {
+  using namespace ic;
+  bool ok = width == 0 || width == 192 || (width >= 16 && width <= 256 && !(width & (width - 1)));
+  ok = ok && swap >= 0 && swap <= 1 && splits >= 1 && splits <= MAX_SPLIT && !(splits & (splits - 1));
+  if (!ok) return fail(IC_ERR_INVALID, "selftest: no such plan");
+  g_plan = Plan{width, swap != 0, splits, 0.0};
   return IC_OK;
 }
 
