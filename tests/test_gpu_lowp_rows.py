@@ -128,3 +128,36 @@ def test_given_row_scales_far_from_one():
         v, s, h = P.decode(q)
         assert np.all(s[:, 0] == 448) and not s[:, 1:].any() and np.all(h == float(np.float32(g)))
         assert np.all(v[:, [3, 5]] == [6, -6]) and np.count_nonzero(v) == 4
+
+
+def test_codes_and_outputs_beyond_32_bits():
+    """Packed codes, int8 codes, values and products that really lie past 2^32 bytes: the last rows against the
+    same rows alone."""
+    last = rows(1, 5, 16384, torch.bfloat16)
+    for make, m in ((lambda t: B.quantize_fp4(t, "nvfp4", rot_size=64), 530000),
+                    (lambda t: B.rmsnorm_quantize(t, torch.ones(16384, device="cuda"))[0], 270000)):
+        x = torch.zeros(m, 16384, dtype=torch.bfloat16, device="cuda")
+        x[-5:] = last
+        q, p = make(x), make(last)
+        del x
+        codes, few = (q.codes, p.codes) if isinstance(q, B.Int8Rows) else (q.packed, p.packed)
+        assert codes.numel() > 2 ** 32 and torch.equal(codes[-5:], few) and not codes[:-5].any()
+        if isinstance(q, B.Int8Rows):
+            v = torch.randint(-5, 6, (40, 16384), device="cuda", dtype=torch.int8)
+            one = torch.ones(40, device="cuda").half()
+            y = B.matmul_int8(q, v, one, out_dtype=torch.float32)
+            assert torch.equal(y[-5:], B.matmul_int8(p, v, one, out_dtype=torch.float32)) and not y[:-5].any()
+            v = B.dequantize_int8(q, torch.float16)
+            assert torch.equal(v[-5:], B.dequantize_int8(p, torch.float16))
+        else:
+            assert all(torch.equal(a[-5:], b) for a, b in zip(parts(q), parts(p)))
+            v = B.dequantize_fp4(q, torch.float16)
+            assert torch.equal(v[-5:], B.dequantize_fp4(p, torch.float16))
+        assert not v[:-5].any()
+        del q, codes, v
+    # y of 5.6 GB; powers of two, so that the sums are exact whatever their order
+    a = torch.exp2(torch.randint(-1, 3, (70000, 64), device="cuda").float())
+    b = torch.exp2(torch.randint(-1, 3, (40000, 64), device="cuda").float())
+    y = B.matmul_fp4(B.quantize_fp4(a), B.quantize_fp4(b))
+    want = (a[-300:].double() @ b.double().T).to(torch.bfloat16)
+    assert y.numel() * 2 > 2 ** 32 and torch.equal(y[-300:], want)
