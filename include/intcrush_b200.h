@@ -379,8 +379,9 @@ enum { IC_INT8 = 0, IC_MXFP4 = 1, IC_NVFP4 = 2 };
  * - 2, -127) + 127.  nvfp4: g = max(amax(row) * (1/2688), 1e-30), or the given
  * row_scale_in (stride 0: one for all rows, 1: one per row; not positive or not
  * finite marks the row); per 16, byte = E4M3(amax * (1/(6g))); codes =
- * E2M1(x * (1/(scale*g))), both reciprocals at most the largest fp32 number.  Codes round to nearest even and saturate at 6.
- * row_scale fp32 [M] is written for nvfp4 only. */
+ * E2M1(x * (1/(scale*g))), where a given g below 2^-118 counts as 2^-118.  Codes
+ * round to nearest even and saturate at 6.  row_scale fp32 [M] is written for
+ * nvfp4 only. */
 int ic_fp4_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, int fmt, int rot,
                     int64_t kp, const float* row_scale_in, int64_t row_scale_stride, uint8_t* packed,
                     uint8_t* scales, float* row_scale, void* stream);

@@ -132,7 +132,6 @@ __device__ __forceinline__ void store16(T* p, int64_t left, const float (&v)[16]
   }
 }
 
-constexpr float F32_MAX = 3.4028234663852886e38f;
 constexpr unsigned INF_BITS = 0x7f800000u;  // |x| as bits: NaN above infinity above every finite value
 
 // max(|a|, |b|, |c|), NaN if one is
@@ -292,7 +291,7 @@ __device__ __forceinline__ void block_scale(unsigned m, const RowScale& rs, uint
   } else {
     bad = m >= INF_BITS || rs.bad;
     byte = bad ? (rs.bad ? 0u : 0x7fu) : to_e4m3(__fmul_rn(__uint_as_float(m), rs.i6g));
-    inv = bad || byte == 0 ? 0.f : fminf(__frcp_rn(__fmul_rn(from_e4m3(byte), rs.s)), F32_MAX);
+    inv = bad || byte == 0 ? 0.f : __frcp_rn(__fmul_rn(from_e4m3(byte), rs.s));
   }
 }
 
@@ -305,8 +304,9 @@ __device__ __forceinline__ void store_fp4(const RowArgs& a, int64_t row, int64_t
   const uint2 codes = make_uint2(e2m1x8(y) & keep, e2m1x8(y + 8) & keep);
   const bool in = row < a.M && c < nch;
   if (in) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.q) + row * a.ldq + c * 8) = codes;
-  // beyond the matrix the norm's 0 times its factor is NaN where that is not finite (a bad row, eps = 0): the bytes there are zero
-  byte = in ? byte : 0u;
+  // beyond the matrix the norm's 0 times its factor is NaN where that is not finite (a bad row, eps = 0): the bytes
+  // there are zero (nvfp4: they are, such a row is bad)
+  if (FMT == IC_MXFP4) byte = in ? byte : 0u;
   uint32_t word;
   int64_t kt;
   bool first;
@@ -552,15 +552,16 @@ __global__ void __launch_bounds__(NP == 2 ? 512 : 256) rows_kernel(const RowArgs
         if (a.row_scale_in) {
           s = row < a.M ? a.row_scale_in[row * a.rs_stride] : 1.f;
           rs.bad = !(s > 0.f) || __float_as_uint(s) >= INF_BITS;
+          // it may be of any size: 1/(scale g) must not be infinite (0 * inf would make codes of zeros), nor 6 g
+          rs.s = fmaxf(s, 0x1p-118f);
+          const float far = s > 0x1p120f ? 0x1p-8f : 1.f;
+          rs.i6g = __fmul_rn(__frcp_rn(__fmul_rn(6.f, __fmul_rn(rs.s, far))), far);
         } else {
           rs.bad = m >= INF_BITS;
           s = fmaxf(__fmul_rn(__uint_as_float(m), (float)(1.0 / 2688.0)), LOWP_SCALE_FLOOR);
+          rs.s = s;
+          rs.i6g = __frcp_rn(__fmul_rn(6.f, s));
         }
-        rs.s = s;
-        // a given scale may be of any size: 6 s stays below infinity, and no reciprocal is infinite (0 * inf would
-        // make codes of zeros); scales in 2^-117..2^120 meet neither
-        const float far = s > 0x1p120f ? 0x1p-8f : 1.f;
-        rs.i6g = fminf(__fmul_rn(__frcp_rn(__fmul_rn(6.f, __fmul_rn(s, far))), far), F32_MAX);
       }
       if (t == 0 && row < a.M) a.row_scale[row] = rs.bad ? __uint_as_float(0x7fc00000u) : s;
     }
