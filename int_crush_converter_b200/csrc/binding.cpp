@@ -1,8 +1,9 @@
 // The short way from torch tensors to the low-precision entry points of
 // libintcrush_b200.so: argument checks, output allocation and the call in one
-// step of native code.  Measured beside a B200: matmul_fp4 5.1 us of host time a
-// call, quantize_fp4 7.2 us; the same steps in Python and ctypes 13.3 and 15.3
-// us, more than most of these kernels run.
+// step of native code, the interpreter's lock released around the last two.
+// Measured beside a B200: matmul_fp4 5.1 us of host time a call, quantize_fp4 7.2
+// us; the same steps in Python and ctypes 13.3 and 15.3 us, more than most of
+// these kernels run.
 //
 // Every function returns None where the arguments are not the ordinary case
 // (tensors on the current CUDA device, of the documented types and layouts) or

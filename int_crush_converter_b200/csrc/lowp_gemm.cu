@@ -19,11 +19,11 @@
 // does not depend on timing.  All waits are bounded (see common.cuh); where one
 // gives up, the elements of y that it leaves without their sums are NaN.
 //
-// Measured on B200 (cuBLAS bf16 1700 TFLOP/s, copy 6.56 TB/s): one row x 12288 x
-// 4096 mxfp4 8.9 us with the weights in HBM, 7.5 us from L2 (25 MB: 4.1 us; a
-// launch and its ends alone take 4.2 us); 512 x 4096 x 4096 mxfp4 9.7 us, 300 x
-// 4096 x 16384 nvfp4 20 us (bound by what L2 delivers to narrow tiles); large
-// products run on CTA pairs, below.
+// Measured on B200 (cuBLAS bf16 1700 TFLOP/s, copy 6.56 TB/s), launches in a
+// graph: one row x 12288 x 4096 mxfp4 9.3 us with the weights in HBM, 7.9 us from
+// L2 (25 MB: 4.1 us; a launch and its ends alone take 4.2 us); 512 x 4096 x 4096
+// mxfp4 9.5 us, 300 x 4096 x 16384 nvfp4 20 us (bound by what L2 delivers to
+// narrow tiles); large products run on CTA pairs, below.
 #include <cstdlib>
 
 #include "internal.h"
@@ -616,12 +616,13 @@ __global__ void __launch_bounds__(256, Cfg<KIND, BN>::CTAS)
 // registers at once and release it; scaling, conversion and stores run under
 // the next products.
 //
-// Measured on B200: 4608 x 16384 x 4096 nvfp4 139 us (4.4 PFLOP/s), 4608 x 4096 x
-// 16384 nvfp4 117 us (5.3), 4608 x 12288 x 4096 int8 150 us (3.1 POP/s), 4608 x
-// 4096 x 16384 int8 200 us (3.1).  Counted in clocks the INT8 main loop runs at
-// 530 a stage of 512 (under the power cap, at 1.5 GHz); the 4-bit ones at 620,
-// because 38 KB a stage is more than five stages in flight bring at L2's latency,
-// and lose 3000 clocks between tiles to the single accumulator.
+// Measured on B200, a few calls at full clocks: 4608 x 16384 x 4096 nvfp4 134 us
+// (4.6 PFLOP/s), 4608 x 4096 x 16384 nvfp4 111 us (5.6), 4608 x 12288 x 4096 int8
+// 149 us (3.1 POP/s), 4608 x 4096 x 16384 int8 200 us (3.1); call after call under
+// the power cap the first takes 168 us (3.7), the third 186 us (2.5).  In clocks
+// the INT8 main loop runs at 530 a stage of 512, the nvfp4 one at 618: 38,912 bytes
+// a stage at the 63 bytes a clock that L2 delivers to an SM.  About 3000 clocks are
+// lost between two tiles of the 4-bit kinds' one accumulator.
 //   full[s]  leader only: the bytes of both CTAs' loads
 //   empty[s] in each CTA: the commit of the products that read the stage
 //   accf[b]  in each CTA: the commit of a tile's last product into accumulator b
@@ -1181,7 +1182,8 @@ void consider(Plan& best, int64_t pm, int64_t qn, int64_t stages, bool swap, boo
 
 template <int KIND>
 Plan plan(int64_t m, int64_t n, int64_t stages, bool aligned) {
-  // pairs: 620 clocks a stage and 3000 between tiles, or an epilogue of element stores; a longer start (measured)
+  // pairs: 620 clocks a stage and 3000 between tiles (nvfp4's, for all kinds: int8 takes 530), or an epilogue of
+  // element stores; a longer start (measured)
   Plan best{0, false, 1, cdiv(cdiv(m, 256) * cdiv(n, 256), 74) * std::max(stages * 620.0 + 3000, aligned ? 0.0 : 18000.0) + 5000};
   for (int swap = 0; swap < 2; ++swap) {
     const int64_t pm = swap ? n : m, qn = swap ? m : n;

@@ -16,12 +16,16 @@
 // each reduction (NP = 0), from L2.  Resident CTAs take rows by turns and load
 // the next ones while they work on these.
 //
-// What bounds them, measured on B200 (copy rate 6.56 TB/s):
-//   quantize 16384 x 4096 bf16   mxfp4 28 us (HBM: 6.1 TB/s), nvfp4 34 us (the row's maximum
-//                                between two barriers), nvfp4 rot256 58 us (shared memory: two
-//                                transposes move 16 bytes an element, 70% of its wavefronts)
-//   norm 4608 x 4096 bf16 with residual   mxfp4 26 us (5.1 TB/s), int8 31 us, nvfp4 rot256 36 us
-//   dequantize 16384 x 4096 nvfp4 to bf16 29 us (5.9 TB/s); one row of 4096: norm 3.9 us
+// What bounds them, measured on B200 (copy rate 6.56 TB/s), calls back to back with the
+// one or two microseconds between them:
+//   quantize 16384 x 4096 bf16   mxfp4 31 us (HBM: 5.5 TB/s), nvfp4 35 us (the row's maximum
+//                                between two barriers), nvfp4 rot256 61 us (two transposes move
+//                                16 bytes an element: 70% of shared memory's wavefronts, with 60%
+//                                of the issue slots and 32% of the warps; none of them a limit)
+//   norm 4608 x 4096 bf16 with residual   mxfp4 28 us (4.4 TB/s), int8 33 us, nvfp4 rot256 39 us
+//   dequantize 16384 x 4096 nvfp4 to bf16 32 us (5.4 TB/s); one row of 4096: norm 4.5 us in a graph
+//   norm 1000 x 12288 bf16 with residual  int8 41 us, mxfp4 rot256 58 us: the instances of the norm
+//                                for 8192 < K <= 32768 spill 0.7 to 4 KB a thread
 // Packed arithmetic, three-input maxima and the transpose are there because the
 // first kernels were bound by instruction issue (80% of the slots, 43
 // instructions an element: 98 us for the rotated nvfp4 case).

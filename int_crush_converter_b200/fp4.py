@@ -154,7 +154,8 @@ def quantize_fp4(x: torch.Tensor, fmt: str = "mxfp4", rot_size: int = 0,
     ``rot_size``: 0, or a power of two: the group Hadamard of ``rotate_weights``
     first, in fp32 (fused for 16..512).  ``row_scale`` (nvfp4): the second-level
     scale, one number for all rows or fp32 [rows]; by default each row's
-    max|x|/2688, so that a row does not depend on its neighbours.  A value that is
+    max|x|/2688, so that a row does not depend on its neighbours (a given one below
+    2^-118 counts as 2^-118 where codes are formed).  A value that is
     not finite marks its mxfp4 block or its nvfp4 row as NaN.
     """
     if row_scale is None and fmt in FORMATS:
@@ -229,7 +230,8 @@ def matmul_fp4(a: FP4Tensor, b: FP4Tensor, bias: torch.Tensor | None = None,
 
     Products of codes and scales are exact, their sums and the bias are held in
     fp32 and rounded once to ``out_dtype`` (fp32/fp16/bf16).  ``b``'s rows are the
-    output's columns.
+    output's columns.  Elements that a wait on the device left without their sum
+    (2 s without progress) are NaN.
     """
     if a.fmt == b.fmt and a.rot_size == b.rot_size and (a.in_features == b.in_features or a.in_features is None or b.in_features is None):
         y = nat.binding().fp4_matmul(a.packed, a.scales, a.row_scale, b.packed, b.scales, b.row_scale, FORMATS.get(a.fmt, 0), bias,

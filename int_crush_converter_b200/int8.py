@@ -120,7 +120,8 @@ def matmul_int8(a: Int8Rows, w_codes: torch.Tensor, w_scales: torch.Tensor,
     ``w_codes``: int8 [N, columns] as the quantizers return them (INT4 codes in
     int8 serve too); ``w_scales``: fp16 [N] or [N, 1]; ``w_zero_points``: int8 or
     None.  Sums are exact in int32 (columns up to 131071, with zero-points 65535),
-    the scaling and the bias fp32, rounded once to ``out_dtype``.  Weights whose
+    the scaling and the bias fp32, rounded once to ``out_dtype``; NaN where a wait
+    on the device gave up, as in ``matmul_fp4``.  Weights whose
     rows are not 16-byte aligned are copied on every call: keep them at such a
     pitch.
     """

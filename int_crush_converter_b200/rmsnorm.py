@@ -22,8 +22,10 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tens
     (:class:`FP4Tensor`, of ``matmul_fp4``).  ``rot_size``: 0 or a power of two in
     16..512, the group Hadamard that the layer's weights were rotated with.
     Returns (quantized rows, h in x's type), h None without a residual.  The sums
-    and the norm are fp32 or wider; a row with a value that is not finite has
-    scale NaN (mxfp4: every block).
+    and the norm are fp32 or wider, and the norm goes on from the fp32 sum
+    x + residual, not from the rounded h that is returned: a layer that norms its
+    rounded stream can get another code where a value lies next to a border.  A
+    row with a value that is not finite has scale NaN (mxfp4: every block).
     """
     if fmt not in _FORMATS:
         raise ValueError(f"fmt must be one of {sorted(_FORMATS)}, got {fmt!r}")
